@@ -36,7 +36,7 @@ enum {
   Q4B_ESTATE = -7        /* object used in the wrong state */
 };
 
-enum { Q4B_F32 = 0, Q4B_F16 = 1 };
+enum { Q4B_F32 = 0, Q4B_F16 = 1, Q4B_BF16 = 2 /* the batched serving operators only */ };
 
 /* Epilogues of q4b_q4_linear:
  *   STORE       y[m, n] = sum_k x[m, k] W[n, k]
@@ -193,6 +193,65 @@ int q4b_silu_mul(const float* gate_up, int rows, int inter, float* out, q4b_stre
 /* Greedy head (:238-239): *index (device int32) = the first index of the largest of logits[n]
  * (torch.argmax's tie rule). */
 int q4b_argmax(const float* logits, int n, int32_t* index, q4b_stream_t stream);
+
+/* ---- batched serving over a paged cache (no reference counterpart: the reference serves one request) ------
+ *
+ * A step of a ragged batch: sequence b of `batch` has the rows q_start[b] .. q_start[b + 1] - 1 of the step
+ * (n_b = 0 allowed), its newest tokens. After the step it holds seq_lens[b] keys of its own, the step's
+ * included: row j of b is key s = seq_lens[b] - n_b + j, kept in slot s % page_size of page
+ * page_table[b, s / page_size], at position prefix_len + s. The prefix_len keys in front are shared by all
+ * sequences (0: none). Device arrays, read when the work runs, so a captured graph follows them; rows
+ * behind q_start[batch] are left as they were. Values are bounded on the device: q_start is clamped to
+ * [0, rows] and to not decrease, seq_lens to the table's keys, and a page id outside [0, n_pages)
+ * holds no keys (appends to it are dropped, attention does not see them). */
+typedef struct q4b_batch {
+  const int32_t* q_start;    /* [batch + 1] */
+  const int32_t* seq_lens;   /* [batch] */
+  const int32_t* page_table; /* [batch, table_width], rows table_stride apart */
+  int batch, table_width;
+  long long table_stride;
+  int prefix_len;
+} q4b_batch;
+
+/* Pools of pages [n_pages, page_size, n_kv_heads, head_dim] of fp16 or bf16 (dtype Q4B_F16 / Q4B_BF16), k
+ * and v with the same strides (elements; multiples of 8, bases 16-byte aligned; head_dim contiguous), so
+ * other orders of page, slot and head are strides too. */
+typedef struct q4b_paged_kv {
+  void* k;
+  void* v;
+  int dtype, n_pages, page_size, n_kv_heads, head_dim;
+  long long page_stride, slot_stride, head_stride;
+} q4b_paged_kv;
+
+/* Appends a step's keys and values to the cache, q and k rotated on the way (the KV write and RoPE of
+ * llama_q4.py:206-223, for a batch). q [rows, n_heads, head_dim], k and v [rows, n_kv_heads, head_dim] of
+ * x_dtype (Q4B_F32, or kv->dtype), rows q_stride / k_stride / v_stride elements apart (multiples of 8), heads
+ * contiguous: parts of one fused projection's rows as they are. cos, sin [table_rows, rot_dim / 2] fp32, rows
+ * rope_stride apart: row p holds position p's angles (whatever scaling they were made with). The first rot_dim
+ * elements of a head turn, pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved; the rest is
+ * copied. head_dim and rot_dim are multiples of 16; rot_dim 0 turns nothing (tables may be NULL).
+ * q_out [rows, n_heads, head_dim] of kv->dtype. Computed in fp32, rounded once. A row whose position the
+ * tables do not reach gets q_out = 0 and appends nothing. Two sequences that append to one slot race. */
+int q4b_paged_rope_append(const void* q, const void* k, const void* v, int x_dtype, long long q_stride,
+                          long long k_stride, long long v_stride, int rows, int n_heads, const float* rope_cos,
+                          const float* rope_sin, long long rope_stride, int table_rows, int rot_dim, int interleaved,
+                          const q4b_batch* batch, const q4b_paged_kv* kv, void* q_out, q4b_stream_t stream);
+
+/* Verification of drafted tokens (the greedy head of llama_q4.py:237-239, for sampling with a draft model).
+ * tokens [rows]: the step's input tokens; row q_start[b] is b's last sure token and the rows behind it
+ * its drafts. Row r of target [rows, vocab] (and of draft, the distributions the drafts were drawn from; NULL:
+ * drafts without one, draft probability 1) predicts tokens[r + 1]. Draft r + 1 is kept while
+ *   uniforms[r] * draft[r, x] < target[r, x],  x = tokens[r + 1];
+ * behind the n_b kept ones a token is drawn from max(target - draft, 0) of row q_start[b] + n_b (draft NULL:
+ * target without x; a residual of zero: target), or, with every draft kept, from the last row's target: the first index whose running
+ * sum exceeds uniforms[last row] * sum. Sums are taken in 64 bits. Probabilities that are negative or not finite
+ * count as zero, a draft outside [0, vocab) is not kept, and weights that are all zero give the token -1.
+ * out_tokens [rows]: at b's rows the kept drafts, the drawn token, then -1; accepted [batch] = n_b (0 for a
+ * sequence without rows). dtype of target and draft: Q4B_F32, Q4B_F16 or Q4B_BF16; rows target_stride /
+ * draft_stride elements apart. vocab <= 2^20. */
+int q4b_verify_drafts(const void* target, const void* draft, int dtype, long long target_stride,
+                      long long draft_stride, int vocab, const int32_t* tokens, const float* uniforms, int rows,
+                      const int32_t* q_start, int batch, int32_t* out_tokens, int32_t* accepted, q4b_stream_t stream);
 
 /* ---- LlamaQ4 model (scripts/llm/llama_q4.py:145-243) --------------------------------------- */
 

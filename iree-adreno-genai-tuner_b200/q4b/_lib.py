@@ -14,6 +14,7 @@ _HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = pathlib.Path(os.environ.get("Q4B_LIB", _HERE / "libq4b.so"))
 
 c_int, c_size_t, c_void_p, c_float, c_char_p = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_float, ctypes.c_char_p
+c_longlong = ctypes.c_longlong
 
 Q4B_OK = 0
 Q4B_EINVAL = -1
@@ -23,7 +24,7 @@ Q4B_ENOMEM = -4
 Q4B_EUNSUPPORTED = -5
 Q4B_ECUDA = -6
 Q4B_ESTATE = -7
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 EPI_STORE, EPI_ACCUMULATE, EPI_SWIGLU = 0, 1, 2
 
 _CODES = {Q4B_EINVAL: "EINVAL", Q4B_ELAUNCH: "ELAUNCH", Q4B_ETIMEOUT: "ETIMEOUT", Q4B_ENOMEM: "ENOMEM",
@@ -57,6 +58,17 @@ class QMat(ctypes.Structure):
 class LayerWeights(ctypes.Structure):
     _fields_ = [("wqkv", QMat), ("wo", QMat), ("wgu", QMat), ("wdown", QMat), ("ln_in", c_void_p),
                 ("ln_post", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p)]
+
+
+class Batch(ctypes.Structure):
+    _fields_ = [("q_start", c_void_p), ("seq_lens", c_void_p), ("page_table", c_void_p), ("batch", c_int),
+                ("table_width", c_int), ("table_stride", ctypes.c_longlong), ("prefix_len", c_int)]
+
+
+class PagedKV(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int), ("n_pages", c_int), ("page_size", c_int),
+                ("n_kv_heads", c_int), ("head_dim", c_int), ("page_stride", ctypes.c_longlong),
+                ("slot_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
 
 
 class RunnerOpts(ctypes.Structure):
@@ -101,6 +113,11 @@ SIGNATURES = {
                                      c_void_p]),
     "q4b_silu_mul": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "q4b_argmax": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
+    "q4b_paged_rope_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_longlong, c_int,
+                                      c_int, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int,
+                                      ctypes.POINTER(Batch), ctypes.POINTER(PagedKV), c_void_p, c_void_p]),
+    "q4b_verify_drafts": (c_int, [c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_int, c_void_p, c_void_p, c_int,
+                                  c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "q4b_tp_init": (c_int, [c_int, c_int, c_void_p, c_int, ctypes.POINTER(c_void_p)]),
     "q4b_tp_destroy": (None, [c_void_p]),
     "q4b_tp_allreduce_f16": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),

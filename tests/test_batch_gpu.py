@@ -1,0 +1,219 @@
+"""GPU parity of the batched serving operators against plain 64-bit implementations (tests/batch_ref.py)."""
+
+import numpy as np
+import pytest
+import torch
+
+import batch_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def q4b():
+    import q4b
+    return q4b
+
+
+def _dev(batch):
+    return {k: R.tensor(batch[k], DEV) for k in ("q_start", "seq_lens", "page_table", "prefix_pages")}
+
+
+def _f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+# ---- paged_rope_append -----------------------------------------------------------------------------------
+
+APPEND = [
+    # lens (new, own), page, prefix, H, Hkv, hd, rot, layout, source, cache
+    ([(1, 1)], 16, 0, 24, 8, 128, 128, "half", "float16", "float16"),
+    ([(1, 600)], 16, 1024, 24, 8, 128, 128, "half", "float32", "float16"),
+    ([(3, 7), (0, 5), (1, 33), (6, 6)], 16, 100, 8, 2, 64, 32, "interleaved", "float32", "bfloat16"),
+    ([(2, 2), (5, 41)], 1, 3, 4, 4, 32, 16, "half", "bfloat16", "bfloat16"),
+    ([(37, 37), (1, 20)], 20, 11, 3, 1, 48, 48, "interleaved", "float16", "float16"),
+    ([(9, 300)], 7, 0, 2, 2, 256, 64, "half", "float16", "float16"),
+    ([(4, 9)], 8, 5, 8, 2, 64, 0, "half", "float32", "float16"),  # nothing turns
+    ([(700, 700), (650, 900)], 64, 77, 4, 1, 64, 64, "half", "bfloat16", "bfloat16"),  # several tokens per CTA
+]
+
+
+def _append_case(lens, page, prefix, H, Hkv, hd, rot, src, cache, seed, spare=0):
+    b = R.make_batch(lens, page, n_pages=sum(-(-o // page) for _, o in lens) + -(-prefix // page) + 3,
+                     prefix_len=prefix, seed=seed, spare_rows=spare)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
+    qkv = rn(b["rows"], (H + 2 * Hkv) * hd).to(getattr(torch, src))
+    q, k, v = (x.view(b["rows"], -1, hd) for x in qkv.split([H * hd, Hkv * hd, Hkv * hd], 1))
+    n_pages = sum(-(-o // page) for _, o in lens) + -(-prefix // page) + 3
+    kp, vp = (rn(n_pages, page, Hkv, hd).to(getattr(torch, cache)) for _ in range(2))
+    cos = sin = None
+    if rot:
+        ang = torch.arange(prefix + max(o for _, o in lens), dtype=torch.float64)[:, None] * \
+            500000.0 ** (-torch.arange(rot // 2, dtype=torch.float64) / (rot // 2))
+        cos, sin = ang.cos().float().to(DEV), ang.sin().float().to(DEV)
+    return b, q, k, v, kp, vp, cos, sin
+
+
+def _close_rounded(got, ref, dtype, terms):
+    """One rounding to dtype (half a step: eps / 2 of the value, or half the smallest subnormal) of an fp32 result
+    whose two products and one sum are each off by at most half an fp32 step of |a c| + |b s| <= terms."""
+    fi = torch.finfo(dtype)
+    tol = fi.eps / 2 * np.abs(ref) * (1 + 2**-20) + 3 * 2.0**-24 * terms + fi.tiny * fi.eps / 2
+    bad = np.abs(got - ref) > tol
+    assert not bad.any(), (np.abs(got - ref)[bad].max(), int(bad.sum()))
+
+
+def _run_append(q4b, case, layout, page, cache, **kw):
+    b, q, k, v, kp, vp, cos, sin = case
+    k0, v0 = _f64(kp), _f64(vp)
+    d = _dev(b)
+    ck, sk = (None, None) if cos is None else (_f64(cos), _f64(sin))
+    ref = R.append(_f64(q), _f64(k), _f64(v), k0, v0, b, ck, sk, layout, page)
+    out = q4b.paged_rope_append(q, k, v, kp, vp, d["page_table"], d["seq_lens"], d["q_start"], cos, sin,
+                                prefix_len=b["prefix_len"], layout=layout, **kw)
+    live = ~np.isnan(ref).any(axis=(1, 2))
+    dt = getattr(torch, cache)
+    _close_rounded(_f64(out)[live], ref[live], dt, 2 * np.abs(_f64(q)).max())
+    _close_rounded(_f64(kp), k0, dt, 2 * np.abs(_f64(k)).max())
+    _close_rounded(_f64(vp), v0, dt, 0.0)
+    return out, live
+
+
+@pytest.mark.parametrize("lens,page,prefix,H,Hkv,hd,rot,layout,src,cache", APPEND)
+def test_append(q4b, lens, page, prefix, H, Hkv, hd, rot, layout, src, cache):
+    _run_append(q4b, _append_case(lens, page, prefix, H, Hkv, hd, rot, src, cache, seed=len(lens)), layout, page, cache)
+
+
+def test_append_leaves_padding_rows_and_other_slots(q4b):
+    """Rows behind the last sequence keep what q_out held; slots of no row keep theirs (checked in _run_append
+    against pools that were written only where the formulas say)."""
+    case = _append_case([(2, 5), (1, 18)], 16, 9, 8, 2, 64, 64, "float16", "float16", 3, spare=4)
+    q_out = torch.full((7, 8, 64), 7.0, dtype=torch.float16, device=DEV)
+    out, live = _run_append(q4b, case, "half", 16, "float16", q_out=q_out)
+    assert out is q_out and live.tolist() == [True] * 3 + [False] * 4
+    assert bool((q_out[3:] == 7.0).all())
+
+
+def test_append_bad_pages_and_far_positions(q4b):
+    """A page id outside the pool drops the append, a position that the tables do not reach gives q_out = 0 and
+    no append; neither touches anything else."""
+    case = list(_append_case([(4, 4), (3, 40), (2, 6)], 4, 2, 4, 2, 32, 32, "float32", "float16", 5))
+    b = case[0]
+    b["page_table"][0, 0] = 10_000
+    b["page_table"][2, 1] = -1
+    case[6], case[7] = case[6][:41], case[7][:41]  # positions 2 + 37 .. 2 + 39: the last one is out
+    out, _ = _run_append(q4b, tuple(case), "half", 4, "float16")
+    assert bool((out[6] == 0).all()) and not bool((out[5] == 0).all())
+
+
+def test_append_other_orders(q4b):
+    """Pools whose pages hold heads before slots, and k and v interleaved in one allocation, are strides."""
+    b, q, k, v, kp, vp, cos, sin = _append_case([(3, 30), (1, 4)], 8, 5, 8, 2, 64, 64, "float16", "float16", 9)
+    both = torch.randn(kp.shape[0], 2, 2, 8, 64, device=DEV).half()  # [page, k|v, head, slot, hd]
+    kp2, vp2 = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    _run_append(q4b, (b, q, k, v, kp2, vp2, cos, sin), "interleaved", 8, "float16")
+
+
+def test_append_uses_the_models_tables(q4b):
+    """cos and sin as q4b.rope_tables makes them (both halves): the first half of the columns, a strided view."""
+    cfg = dict(hidden_size=512, num_attention_heads=8, num_key_value_heads=2, head_dim=64, rope_theta=500000.0,
+               max_position_embeddings=4096)
+    cos, sin = (x.to(DEV)[:, :32] for x in q4b.rope_tables(cfg, 64))
+    b, q, k, v, kp, vp, _, _ = _append_case([(3, 30), (1, 4)], 8, 5, 8, 2, 64, 64, "float32", "float16", 9)
+    _run_append(q4b, (b, q, k, v, kp, vp, cos, sin), "half", 8, "float16")
+
+
+# ---- verify_drafts ---------------------------------------------------------------------------------------
+
+
+def _verify_case(news, vocab, dtype, drafts, seed, sharp=2.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    rows = sum(news)
+    logits = sharp * torch.randn(rows, vocab, generator=g, device=DEV)
+    noisy = logits + 0.8 * torch.randn(rows, vocab, generator=g, device=DEV)
+    target, draft = torch.softmax(logits, -1), torch.softmax(noisy, -1)
+    drawn = torch.multinomial(draft, 1, generator=g)[:, 0].int() if vocab < 2**24 else None
+    tokens = torch.cat([drawn[:1], drawn[:-1]])
+    q_start = torch.from_numpy(np.concatenate([[0], np.cumsum(news)]).astype(np.int32)).to(DEV)
+    return (target.to(dtype), draft.to(dtype) if drafts else None, tokens,
+            torch.rand(rows, generator=g, device=DEV), q_start)
+
+
+def _run_verify(q4b, case, **kw):
+    target, draft, tokens, uniforms, q_start = case
+    got, acc = q4b.verify_drafts(target, draft, tokens, uniforms, q_start, **kw)
+    n = lambda t: t.detach().float().cpu().numpy()  # noqa: E731
+    ref, racc = R.verify(n(target), None if draft is None else n(draft), tokens.cpu().numpy(), n(uniforms),
+                         q_start.cpu().numpy())
+    assert acc.tolist() == racc
+    for r, x in enumerate(ref):
+        if x is not None:
+            assert int(got[r]) == x, r
+    return got, acc, ref
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("drafts", [True, False])
+@pytest.mark.parametrize("news,vocab", [([1], 1), ([5], 7), ([3, 1, 0, 6, 2], 1000), ([5] * 3, 32064), ([40, 33], 501),
+                                        ([2, 8, 1], 128256), ([3] * 160, 1025), ([4, 4], 49999)])
+def test_verify(q4b, news, vocab, drafts, dtype):
+    case = _verify_case(news, vocab, getattr(torch, dtype), drafts, seed=vocab + len(news))
+    _run_verify(q4b, case)
+
+
+def test_verify_keeps_every_share(q4b):
+    """Over many sequences all lengths of the kept run occur, and the drawn tokens differ from rejected ones."""
+    case = _verify_case([4] * 400, 300, torch.float32, True, 11)
+    got, acc, _ = _run_verify(q4b, case)
+    assert set(acc.tolist()) == {0, 1, 2, 3}
+
+
+def test_verify_edges(q4b):
+    v = 4096
+    u = lambda *x: torch.tensor(x, dtype=torch.float32, device=DEV)  # noqa: E731
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    one = torch.zeros(2, v, device=DEV)
+    one[:, 5] = 1.0
+    # target == draft: always kept (u < 1); then a draw from a single spike, at u = 0 and at the largest u below 1
+    for x in (0.0, float(np.nextafter(np.float32(1), np.float32(0)))):
+        got, acc, _ = _run_verify(q4b, (one, one, i(0, 5), u(x, x), i(0, 2)))
+        assert got.tolist() == [5, 5] and acc.tolist() == [1]
+    # a draft of zero probability in both, with an empty residual: rejected, drawn from the target
+    got, acc, _ = _run_verify(q4b, (one, one, i(0, 6), u(0.0, 0.5), i(0, 2)))
+    assert got.tolist() == [5, -1] and acc.tolist() == [0]
+    # drafts outside the vocabulary are not kept
+    for x in (-1, v, 2**31 - 1):
+        got, acc, _ = _run_verify(q4b, (one, None, i(0, x), u(0.0, 0.5), i(0, 2)))
+        assert got.tolist() == [5, -1]
+    # no weight anywhere: the token -1; NaN, infinite and negative probabilities count as zero
+    zero = torch.zeros(1, v, device=DEV)
+    zero[0, 7], zero[0, 8], zero[0, 9] = float("nan"), float("inf"), -1.0
+    got, acc, _ = _run_verify(q4b, (zero, None, i(0), u(0.5), i(0, 1)))
+    assert got.tolist() == [-1]
+    zero[0, 4000] = 1e-30
+    got, acc, _ = _run_verify(q4b, (zero, None, i(0), u(0.5), i(0, 1)))
+    assert got.tolist() == [4000]
+
+
+def test_verify_padding_and_strides(q4b):
+    """Rows behind the last sequence keep what out held; rows of a wider buffer, p and d aligned differently."""
+    target, draft, tokens, uniforms, q_start = _verify_case([3, 2], 1003, torch.float32, True, 4)
+    wide = torch.full((8, 1010), float("nan"), device=DEV)
+    tw, dw = wide[:, 1:1004], wide.clone()[:, 2:1005]
+    tw[:5], dw[:5] = target, draft
+    tok = torch.cat([tokens, tokens[:3]])
+    uni = torch.cat([uniforms, uniforms[:3]])
+    out = torch.full((8,), 77, dtype=torch.int32, device=DEV)
+    got, acc, ref = _run_verify(q4b, (tw, dw, tok, uni, q_start), out=out)
+    assert got is out and got[5:].tolist() == [77] * 3 and ref[5:] == [None] * 3
+
+
+def test_verify_malformed_offsets_stay_in_bounds(q4b):
+    """q_start beyond the rows or decreasing is clamped on the device: no row outside is touched."""
+    target, draft, tokens, uniforms, _ = _verify_case([3, 3], 257, torch.float32, True, 6)
+    for bad in ([0, 3, 900], [0, 5, 2], [-4, 3, 6], [9, 9, 9]):
+        q_start = torch.tensor(bad, dtype=torch.int32, device=DEV)
+        _, acc = q4b.verify_drafts(target, draft, tokens, uniforms, q_start)
+        assert all(0 <= a <= 6 for a in acc.tolist())
