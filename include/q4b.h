@@ -201,8 +201,8 @@ int q4b_argmax(const float* logits, int n, int32_t* index, q4b_stream_t stream);
  * included: row j of b is key s = seq_lens[b] - n_b + j, kept in slot s % page_size of page
  * page_table[b, s / page_size], at position prefix_len + s. The prefix_len keys in front are shared by all
  * sequences (0: none). Device arrays, read when the work runs, so a captured graph follows them; rows
- * behind q_start[batch] are left as they were. Values are bounded on the device: q_start is clamped to
- * [0, rows] and to not decrease, seq_lens to the table's keys, and a page id outside [0, n_pages)
+ * behind q_start[batch] are left as they were. Values are bounded on the device: q_start (which must
+ * not decrease) is clamped to [0, rows], seq_lens to the table's keys, and a page id outside [0, n_pages)
  * holds no keys (appends to it are dropped, attention does not see them). */
 typedef struct q4b_batch {
   const int32_t* q_start;    /* [batch + 1] */
@@ -236,6 +236,19 @@ int q4b_paged_rope_append(const void* q, const void* k, const void* v, int x_dty
                           long long k_stride, long long v_stride, int rows, int n_heads, const float* rope_cos,
                           const float* rope_sin, long long rope_stride, int table_rows, int rot_dim, int interleaved,
                           const q4b_batch* batch, const q4b_paged_kv* kv, void* q_out, q4b_stream_t stream);
+
+/* Attention of a step over the shared prefix and each sequence's own keys (the GQA attention of
+ * llama_q4.py:208-232, for a batch): row j of b sees the prefix_len keys in the pages prefix_pages[0 ..
+ * ceil(prefix_len / page_size) - 1] (device) and its own keys 0 .. seq_lens[b] - n_b + j, and is zero if
+ * there are none. q [rows, n_heads, head_dim] of kv->dtype, rotated, rows q_stride and heads q_head_stride
+ * elements apart (even); out [rows, n_heads * head_dim] of kv->dtype; scale > 0 (1 / sqrt(head_dim)).
+ * The prefix is read once for all sequences. fp32 scores, sums and weighted V; weights enter the PV
+ * product rounded to kv->dtype. head_dim 32, 64 or 128; batch <= 4096. The workspace (256-byte aligned) needs no
+ * initialisation and holds nothing between calls; calls that share one must not overlap. */
+size_t q4b_prefix_attention_workspace(int rows, int n_heads, const q4b_batch* batch, const q4b_paged_kv* kv);
+int q4b_prefix_attention(const void* q, long long q_stride, long long q_head_stride, int rows, int n_heads,
+                         float scale, const int32_t* prefix_pages, const q4b_batch* batch, const q4b_paged_kv* kv,
+                         void* out, void* workspace, size_t workspace_bytes, q4b_stream_t stream);
 
 /* Verification of drafted tokens (the greedy head of llama_q4.py:237-239, for sampling with a draft model).
  * tokens [rows]: the step's input tokens; row q_start[b] is b's last sure token and the rows behind it

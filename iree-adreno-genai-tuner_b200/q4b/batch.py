@@ -129,6 +129,42 @@ def paged_rope_append(q, k, v, k_pages, v_pages, page_table, seq_lens, q_start, 
     return q_out
 
 
+def prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, page_table, seq_lens, q_start, *,
+                     scale=None, out=None):
+    """Attention of a step's rows over the shared prefix and each sequence's own keys -> [rows, H * hd].
+
+    q [rows, H, hd] of the cache's type, rotated (any row and head stride); prefix_pages int32: the pages
+    of the prefix_len shared keys (prefix_len 0: none, every sequence on its own). Row j of sequence b sees the
+    prefix and b's own keys up to its own; a row that sees none is zero. The prefix is read
+    once for all sequences. scale defaults to 1 / sqrt(hd). head_dim 32, 64 or 128."""
+    what = "prefix_attention"
+    dev = _same_device(what, q=q, k_pages=k_pages, v_pages=v_pages, prefix_pages=prefix_pages, page_table=page_table,
+                       seq_lens=seq_lens, q_start=q_start, out=out)
+    kv = _paged_kv(what, k_pages, v_pages)
+    batch = _batch(what, q_start, seq_lens, page_table, prefix_len)
+    _int32(what, "prefix_pages", prefix_pages, 1)
+    if prefix_pages.shape[0] * kv.page_size < prefix_len:
+        raise ValueError(f"{what}: {prefix_pages.shape[0]} prefix pages of {kv.page_size} hold no {prefix_len} keys")
+    if q.dim() != 3 or q.shape[2] != kv.head_dim or q.dtype != k_pages.dtype or (q.numel() and q.stride(2) != 1):
+        raise ValueError(f"{what}: q must be [rows, heads, {kv.head_dim}] of the cache's type, head_dim contiguous")
+    rows, H, hd = q.shape
+    if out is None:
+        out = torch.empty(rows, H * hd, dtype=q.dtype, device=dev)
+    elif out.shape != (rows, H * hd) or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be a contiguous {q.dtype} [{rows}, {H * hd}] tensor")
+    if rows == 0:
+        return out
+    L, bp, kp = lib(), ctypes.byref(batch), ctypes.byref(kv)
+    with _on(dev):
+        # made anew for each call: the allocator keeps streams and captured graphs apart
+        ws = torch.empty(L.q4b_prefix_attention_workspace(rows, H, bp, kp), dtype=torch.uint8, device=dev)
+        check(L.q4b_prefix_attention(q.data_ptr(), q.stride(0), q.stride(1), rows, H,
+                                     1.0 / math.sqrt(hd) if scale is None else scale, prefix_pages.data_ptr(), bp, kp,
+                                     out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                     torch.cuda.current_stream().cuda_stream), what)
+    return out
+
+
 def verify_drafts(target, draft, tokens, uniforms, q_start, *, out=None):
     """Verify drafted tokens against the target's probabilities; returns (tokens [rows], accepted [B]) int32.
 

@@ -125,6 +125,174 @@ def test_append_uses_the_models_tables(q4b):
     _run_append(q4b, (b, q, k, v, kp, vp, cos, sin), "half", 8, "float16")
 
 
+# ---- prefix_attention ------------------------------------------------------------------------------------
+
+ATTEND = [
+    # lens (new, own), page, prefix, H, Hkv, hd
+    ([(1, 1)], 16, 0, 24, 8, 128),
+    ([(1, 60), (1, 33)], 16, 250, 24, 8, 128),
+    ([(1, 0), (0, 9), (1, 1), (1, 64), (1, 65)], 16, 1, 8, 2, 64),  # no own keys, no rows, tile borders
+    ([(3, 2), (4, 4), (2, 130)], 8, 0, 6, 1, 64),  # more rows than keys: rows that see nothing
+    ([(1, 500)] * 3 + [(1, 3)], 1, 129, 8, 2, 32),
+    ([(5, 77), (1, 300), (7, 7)], 20, 63, 32, 4, 64),
+    ([(40, 200), (33, 33), (1, 900)], 64, 1000, 3, 1, 128),  # several row tiles, causal inside
+    ([(1, 1)] * 70, 16, 513, 8, 8, 128),  # more than one row tile of the prefix, one head per KV head
+    ([(2, 2000)], 16, 3000, 8, 2, 128),
+    ([(130, 130), (100, 700)], 16, 300, 4, 4, 32),
+]
+
+
+def _attend_case(lens, page, prefix, H, Hkv, hd, dtype, seed, spare=0, sharp=1.0):
+    n_pages = sum(-(-o // page) for _, o in lens) + -(-prefix // page) + 2
+    b = R.make_batch(lens, page, n_pages, prefix_len=prefix, seed=seed, spare_rows=spare)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
+    q = (sharp * rn(b["rows"], H, hd)).to(dtype)
+    kp, vp = (rn(n_pages, page, Hkv, hd).to(dtype) for _ in range(2))
+    # slots that no sequence holds: what a fresh or reused pool may contain
+    held = np.zeros((n_pages, page), dtype=bool)
+    for pages, n in [(b["prefix_pages"], prefix)] + [(b["page_table"][i], o) for i, (_, o) in enumerate(lens)]:
+        for s in range(n):
+            held[pages[s // page], s % page] = True
+    free = torch.from_numpy(~held).to(DEV)
+    kp[free], vp[free] = float("nan"), float("inf")
+    return b, q, kp, vp
+
+
+def _check_attend(got, ref, vp, dtype, live):
+    """Output rounding: half a step of the value. P rounding: each weight is off by at most half a step of itself
+    (fp16: or half the smallest subnormal), so the weighted mean by eps / 2 * sum(w |v|) <= eps / 2 * max|v|. fp32
+    sums and exponentials of scores |s| < 60: below 2^-15 of max|v|."""
+    fi = torch.finfo(dtype)
+    vmax = np.nanmax(np.abs(np.where(np.isfinite(vp), vp, np.nan)), initial=1.0)
+    tol = fi.eps / 2 * np.abs(ref) + (fi.eps / 2 + 2.0**-15) * vmax + fi.tiny * fi.eps
+    err = np.abs(got - ref)
+    assert np.array_equal(np.isnan(got), np.isnan(ref)) and not (err[live] > tol[live]).any(), np.nanmax(err[live])
+    # the bound above is for the worst case; rounding errors of many keys are independent
+    if live.any() and np.abs(ref[live]).max() > 0:
+        assert np.linalg.norm(err[live]) <= 2 * fi.eps / 2 * np.linalg.norm(ref[live]) + 2.0**-15
+
+
+def _run_attend(q4b, case, page, **kw):
+    b, q, kp, vp = case
+    d = _dev(b)
+    ref = R.attention(_f64(q), _f64(kp), _f64(vp), b, page, scale=kw.get("scale"))
+    out = q4b.prefix_attention(q, kp, vp, d["prefix_pages"], b["prefix_len"], d["page_table"], d["seq_lens"],
+                               d["q_start"], **kw)
+    live = ~np.isnan(ref).any(axis=(1, 2))
+    got = _f64(out).reshape(ref.shape)
+    _check_attend(np.where(live[:, None, None], got, 0), np.where(live[:, None, None], ref, 0), _f64(vp), q.dtype, live)
+    return out, ref, live
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,page,prefix,H,Hkv,hd", ATTEND)
+def test_attend(q4b, lens, page, prefix, H, Hkv, hd, dtype):
+    _, _, live = _run_attend(q4b, _attend_case(lens, page, prefix, H, Hkv, hd, dtype, seed=len(lens) + prefix), page)
+    assert live.all()
+
+
+def test_attend_rows_without_keys_are_zero(q4b):
+    out, ref, _ = _run_attend(q4b, _attend_case([(3, 1), (2, 0), (1, 5)], 4, 0, 4, 2, 64, torch.float16, 3), 4)
+    assert bool((out[:2] == 0).all()) and bool((out[3:5] == 0).all()) and not bool((out[2] == 0).all())
+
+
+def test_attend_leaves_padding_rows(q4b):
+    case = _attend_case([(2, 5), (1, 18)], 16, 40, 8, 2, 64, torch.bfloat16, 3, spare=3)
+    case[1][3:] = float("nan")
+    out = torch.full((6, 512), 7.0, dtype=torch.bfloat16, device=DEV)
+    got, _, live = _run_attend(q4b, case, 16, out=out)
+    assert got is out and live.tolist() == [True] * 3 + [False] * 3 and bool((out[3:] == 7.0).all())
+
+
+def test_attend_bad_pages_hold_no_keys(q4b):
+    case = _attend_case([(1, 70), (3, 40), (1, 8)], 8, 100, 8, 2, 64, torch.float16, 5)
+    case[0]["page_table"][0, 3], case[0]["page_table"][1, 4], case[0]["prefix_pages"][7] = -1, 10**6, 2**31 - 1
+    case[0]["page_table"][2, 0] = -2**31
+    _run_attend(q4b, case, 8)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new,own,g", [(4, 20, 4), (4, 4, 1), (60, 100, 3)])
+def test_attend_later_keys_do_not_leak(q4b, value, dtype, new, own, g):
+    """A draft whose k or v overflowed spoils its own row and later ones, and no earlier row."""
+    for which in (0, 1):
+        case = _attend_case([(new, own), (2, 9)], 8, 30, 2 * g, 2, 64, dtype, 7)
+        b, q, kp, vp = case
+        bad = own - new + 2  # key of row 2
+        (kp, vp)[which][b["page_table"][0, bad // 8], bad % 8] = value
+        d = _dev(b)
+        out = _f64(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 30, d["page_table"], d["seq_lens"], d["q_start"]))
+        clean = [t for t in range(b["rows"]) if t < 2 or t >= new]
+        with np.errstate(all="ignore"):
+            ref = R.attention(_f64(q), _f64(kp), _f64(vp), b, 8).reshape(out.shape)
+        live = np.zeros(b["rows"], dtype=bool)
+        live[clean] = True
+        _check_attend(np.where(live[:, None], out, 0), np.where(live[:, None], ref, 0), _f64(vp), dtype, live)
+        if which == 1:
+            assert not np.isfinite(out[2:new]).any()
+
+
+def test_attend_strides_scale_and_orders(q4b):
+    """q as a part of wider rows and head-major, pools with heads before slots, another scale."""
+    b, q, kp, vp = _attend_case([(3, 30), (1, 44)], 8, 50, 8, 2, 64, torch.float16, 9)
+    both = torch.randn(kp.shape[0], 2, 2, 8, 64, device=DEV).half()
+    kp2, vp2 = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    kp2.copy_(kp), vp2.copy_(vp)
+    wide = torch.randn(4, 9 * 64 + 6, device=DEV).half()
+    q2 = wide[:, 2:2 + 512].view(4, 8, 64)
+    q2.copy_(q)
+    _run_attend(q4b, (b, q2, kp2, vp2), 8, scale=0.05)
+    q3 = q.transpose(0, 1).contiguous().transpose(0, 1)
+    _run_attend(q4b, (b, q3, kp2, vp2), 8)
+
+
+def test_attend_sharp_scores(q4b):
+    """Scores of some hundreds: the running maximum does the work."""
+    _run_attend(q4b, _attend_case([(2, 300), (1, 31)], 16, 700, 8, 2, 64, torch.float16, 9, sharp=3.0), 16, scale=2.0)
+
+
+def test_attend_far_pages(q4b):
+    """Element offsets behind 2^32 in the pool."""
+    n_pages, page, Hkv, hd = 70_000, 64, 8, 128  # 4.6e9 elements, 9 GB each
+    kp = torch.empty(n_pages, page, Hkv, hd, dtype=torch.float16, device=DEV)
+    vp = torch.empty_like(kp)
+    b = R.make_batch([(2, 150)], page, 6, prefix_len=100)
+    far = np.array([69_999, 3, 65_537, 40_000, 68_000, 66_000])
+    for name in ("page_table", "prefix_pages"):
+        b[name] = far[b[name]].astype(np.int32)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    small_k, small_v = (torch.randn(6, page, Hkv, hd, generator=g, device=DEV).half() for _ in range(2))
+    at = torch.from_numpy(far).to(DEV)
+    kp[at], vp[at] = small_k, small_v
+    q = torch.randn(2, 16, hd, generator=g, device=DEV).half()
+    d = _dev(b)
+    out = _f64(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 100, d["page_table"], d["seq_lens"], d["q_start"]))
+    back = {int(x): i for i, x in enumerate(far)}
+    b2 = dict(b, page_table=np.vectorize(back.get)(b["page_table"]), prefix_pages=np.vectorize(back.get)(b["prefix_pages"]))
+    ref = R.attention(_f64(q), _f64(small_k), _f64(small_v), b2, page)
+    _check_attend(out.reshape(ref.shape), ref, _f64(small_v), torch.float16, np.ones(2, dtype=bool))
+    # and the append reaches them
+    x = torch.randn(2, 2 * Hkv, hd, device=DEV).half()
+    q4b.paged_rope_append(q, x[:, :Hkv], x[:, Hkv:], kp, vp, d["page_table"], d["seq_lens"], d["q_start"], prefix_len=100)
+    for j, s in enumerate((148, 149)):
+        page_id = int(b["page_table"][0, s // page])
+        assert torch.equal(kp[page_id, s % page], x[j, :Hkv]) and torch.equal(vp[page_id, s % page], x[j, Hkv:])
+    del kp, vp
+    torch.cuda.empty_cache()
+
+
+def test_attend_malformed_offsets_stay_in_bounds(q4b):
+    b, q, kp, vp = _attend_case([(3, 30), (3, 44)], 8, 50, 8, 2, 64, torch.float16, 9)
+    d = _dev(b)
+    for bad in ([0, 3, 900], [0, 5, 2], [-4, 3, 6], [9, 9, 9]):
+        q_start = torch.tensor(bad, dtype=torch.int32, device=DEV)
+        lens = torch.tensor([2**31 - 1, -5], dtype=torch.int32, device=DEV)
+        q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 50, d["page_table"], lens, q_start)
+    torch.cuda.synchronize()
+
+
 # ---- verify_drafts ---------------------------------------------------------------------------------------
 
 
