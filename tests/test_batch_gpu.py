@@ -385,3 +385,155 @@ def test_verify_malformed_offsets_stay_in_bounds(q4b):
         q_start = torch.tensor(bad, dtype=torch.int32, device=DEV)
         _, acc = q4b.verify_drafts(target, draft, tokens, uniforms, q_start)
         assert all(0 <= a <= 6 for a in acc.tolist())
+
+
+# ---- the wrappers' refusals, streams, graphs, and a step of them all ---------------------------------------
+
+
+def test_wrappers_refuse(q4b):
+    case = _append_case([(2, 5), (1, 18)], 16, 9, 8, 2, 64, 64, "float16", "float16", 3)
+    b, q, k, v, kp, vp, cos, sin = case
+    d = _dev(b)
+    meta = (d["page_table"], d["seq_lens"], d["q_start"])
+    ap = lambda *a, **kw: q4b.paged_rope_append(*a, **{"prefix_len": 9, **kw})  # noqa: E731
+    at = lambda *a, **kw: q4b.prefix_attention(*a, **kw)  # noqa: E731
+    q16 = q.contiguous()
+    bad = [
+        (ValueError, "cache's type", lambda: ap(q.bfloat16(), k.bfloat16(), v.bfloat16(), kp, vp, *meta, cos, sin)),
+        (ValueError, "same rows", lambda: ap(q, k[:2], v, kp, vp, *meta, cos, sin)),
+        (ValueError, "must be \\[rows", lambda: ap(q, k[:, :1], v, kp, vp, *meta, cos, sin)),
+        (ValueError, "contiguous", lambda: ap(q.transpose(0, 1).contiguous().transpose(0, 1), k, v, kp, vp, *meta, cos, sin)),
+        (ValueError, "together", lambda: ap(q, k, v, kp, vp, *meta, cos, None)),
+        (ValueError, "layout", lambda: ap(q, k, v, kp, vp, *meta, cos, sin, layout="both")),
+        (ValueError, "fp32 \\[positions", lambda: ap(q, k, v, kp, vp, *meta, cos.half(), sin.half())),
+        (ValueError, "same strides", lambda: ap(q, k, v, kp, vp.transpose(1, 2).contiguous().transpose(1, 2), *meta, cos, sin)),
+        (ValueError, "int32", lambda: ap(q, k, v, kp, vp, meta[0].long(), *meta[1:], cos, sin)),
+        (ValueError, "seq_lens need", lambda: ap(q, k, v, kp, vp, meta[0], meta[1], meta[2][:-1], cos, sin)),
+        (ValueError, "out of range", lambda: ap(q, k, v, kp, vp, *meta, cos, sin, prefix_len=-1)),
+        (ValueError, "integer", lambda: ap(q, k, v, kp, vp, *meta, cos, sin, prefix_len="9")),
+        (ValueError, "CUDA", lambda: ap(q, k, v, kp, vp, meta[0].cpu(), *meta[1:], cos, sin)),
+        (ValueError, "q_out", lambda: ap(q, k, v, kp, vp, *meta, cos, sin, q_out=q16.float())),
+        (q4b.Q4BError, "rot_dim", lambda: ap(q, k, v, kp, vp, *meta, cos[:, :4], sin[:, :4])),
+        (ValueError, "tensor", lambda: at(None, kp, vp, d["prefix_pages"], 9, *meta)),
+        (ValueError, "hold no", lambda: at(q16, kp, vp, d["prefix_pages"], 17, *meta)),
+        (ValueError, "cache's type", lambda: at(q16.float(), kp, vp, d["prefix_pages"], 9, *meta)),
+        (ValueError, "out must", lambda: at(q16, kp, vp, d["prefix_pages"], 9, *meta, out=q16)),
+        (q4b.Q4BError, "scale", lambda: at(q16, kp, vp, d["prefix_pages"], 9, *meta, scale=0.0)),
+        (TypeError, "number", lambda: at(q16, kp, vp, d["prefix_pages"], 9, *meta, scale="x")),
+        (q4b.Q4BError, "head_dim", lambda: at(q16[..., :48], kp[..., :48], vp[..., :48], d["prefix_pages"], 9, *meta)),
+        (q4b.Q4BError, "n_kv_heads", lambda: at(q16[:, :3], kp, vp, d["prefix_pages"], 9, *meta)),
+    ]
+    t, dr, tok, u, qs = _verify_case([3, 2], 100, torch.float32, True, 1)
+    bad += [
+        (ValueError, "like target", lambda: q4b.verify_drafts(t, dr.half(), tok, u, qs)),
+        (ValueError, "like target", lambda: q4b.verify_drafts(t, dr[:, :50], tok, u, qs)),
+        (ValueError, "rows need", lambda: q4b.verify_drafts(t, dr, tok[:4], u, qs)),
+        (ValueError, "rows need", lambda: q4b.verify_drafts(t, dr, tok, u.double(), qs)),
+        (ValueError, "int32", lambda: q4b.verify_drafts(t, dr, tok.long(), u, qs)),
+        (ValueError, "last dimension", lambda: q4b.verify_drafts(t.t().contiguous().t(), dr, tok, u, qs)),
+        (ValueError, "out", lambda: q4b.verify_drafts(t, dr, tok, u, qs, out=tok[:3])),
+    ]
+    for kind, word, call in bad:
+        with pytest.raises(kind, match=word):
+            call()
+
+
+def test_empty_steps(q4b):
+    b, q, k, v, kp, vp, cos, sin = _append_case([(2, 5)], 16, 9, 8, 2, 64, 64, "float16", "float16", 3)
+    d = _dev(b)
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert q4b.paged_rope_append(q[:0], k[:0], v[:0], kp, vp, d["page_table"], d["seq_lens"], d["q_start"], cos,
+                                 sin).shape == (0, 8, 64)
+    assert q4b.prefix_attention(q[:0], kp, vp, d["prefix_pages"], 9, d["page_table"][:0], d["seq_lens"][:0], none).shape == (0, 512)
+    t, acc = q4b.verify_drafts(torch.zeros(0, 9, device=DEV), None, none[:0], torch.zeros(0, device=DEV), none)
+    assert t.numel() == 0 and acc.numel() == 0
+    zeros = torch.zeros(4, dtype=torch.int32, device=DEV)  # sequences without rows
+    t, acc = q4b.verify_drafts(torch.zeros(0, 9, device=DEV), None, none[:0], torch.zeros(0, device=DEV), zeros)
+    assert acc.tolist() == [0, 0, 0]
+
+
+def _step(q4b, s, out=None):
+    """append -> attention -> (a stand-in for the rest of the model) -> verification."""
+    q = q4b.paged_rope_append(s["q"], s["k"], s["v"], s["kp"], s["vp"], s["table"], s["lens"], s["q_start"], s["cos"],
+                              s["sin"], prefix_len=s["prefix"])
+    o = q4b.prefix_attention(q, s["kp"], s["vp"], s["pages"], s["prefix"], s["table"], s["lens"], s["q_start"])
+    target = torch.softmax(o.float() @ s["head"], -1)
+    return (q, o) + q4b.verify_drafts(target, s["draft"], s["tokens"], s["uniforms"], s["q_start"])
+
+
+def _step_case(seed, vocab=500):
+    b, q, k, v, kp, vp, cos, sin = _append_case([(3, 30), (1, 44), (5, 5), (2, 100)], 8, 50, 8, 2, 64, 64, "float32",
+                                                "float16", seed)
+    g = torch.Generator(device=DEV).manual_seed(seed + 100)
+    d = _dev(b)
+    draft = torch.softmax(torch.randn(11, vocab, generator=g, device=DEV), -1)
+    return dict(b=b, q=q, k=k, v=v, kp=kp, vp=vp, cos=cos, sin=sin, table=d["page_table"], lens=d["seq_lens"],
+                q_start=d["q_start"], pages=d["prefix_pages"], prefix=50, draft=draft,
+                head=0.3 * torch.randn(512, vocab, generator=g, device=DEV),
+                tokens=torch.randint(0, vocab, (11,), generator=g, device=DEV, dtype=torch.int32),
+                uniforms=torch.rand(11, generator=g, device=DEV))
+
+
+def test_step_of_a_batch(q4b):
+    """The operators in a row, as a serving step runs them, against the plain forms on the way."""
+    s = _step_case(21)
+    k0, v0 = _f64(s["kp"]), _f64(s["vp"])
+    ref_q = R.append(_f64(s["q"]), _f64(s["k"]), _f64(s["v"]), k0, v0, s["b"], _f64(s["cos"]), _f64(s["sin"]), "half", 8)
+    q, o, toks, acc = _step(q4b, s)
+    _close_rounded(_f64(q), ref_q, torch.float16, 2 * np.abs(_f64(s["q"])).max())
+    ref = R.attention(_f64(q), _f64(s["kp"]), _f64(s["vp"]), s["b"], 8)
+    _check_attend(_f64(o).reshape(ref.shape), ref, _f64(s["vp"]), torch.float16, np.ones(11, dtype=bool))
+    target = torch.softmax(o.float() @ s["head"], -1).cpu().numpy()
+    rt, ra = R.verify(target, s["draft"].cpu().numpy(), s["tokens"].cpu().numpy(), s["uniforms"].cpu().numpy(),
+                      s["b"]["q_start"])
+    assert toks.tolist() == rt and acc.tolist() == ra
+
+
+def test_step_in_graphs_and_streams(q4b):
+    """Two captured steps replayed on two streams at once, with new contents in the same tensors, give what eager
+    calls give; a graph follows lengths and offsets that change between replays."""
+    cases = [_step_case(31), _step_case(32)]
+    graphs, outs = [], []
+    for s in cases:
+        _step(q4b, s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_step(q4b, s))
+        graphs.append(g)
+    for s, n in zip(cases, (33, 34)):
+        new = _step_case(n)
+        for name in ("q", "k", "v", "kp", "vp", "draft", "tokens", "uniforms", "head"):
+            s[name].copy_(new[name])
+        s["lens"].copy_(torch.tensor([17, 40, 5, 93], dtype=torch.int32))
+        s["q_start"].copy_(torch.tensor([0, 1, 4, 6, 9], dtype=torch.int32))
+    eager = []
+    for s in cases:
+        kp, vp = s["kp"].clone(), s["vp"].clone()
+        eager.append([x.clone() for x in _step(q4b, s)] + [s["kp"].clone(), s["vp"].clone()])
+        s["kp"].copy_(kp), s["vp"].copy_(vp)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for s, out, ref in zip(cases, outs, eager):
+        for x, y in zip(list(out) + [s["kp"], s["vp"]], ref):
+            live = slice(0, 9) if x.shape[0] == 11 else slice(None)
+            assert torch.equal(x[live], y[live])
+
+
+def test_results_do_not_depend_on_timing(q4b):
+    """The same call gives the same bits, whatever runs beside it."""
+    s = _step_case(41)
+    first = _step(q4b, s)
+    side = torch.cuda.Stream()
+    noise = torch.randn(4096, 4096, device=DEV)
+    for _ in range(10):
+        with torch.cuda.stream(side):
+            noise @ noise
+        for x, y in zip(first, _step(q4b, s)):
+            assert torch.equal(x, y)
+    torch.cuda.synchronize()
