@@ -761,6 +761,24 @@ int make_tmap_i32(CUtensorMap* map, const void* base, uint64_t cols, uint64_t ro
   return Q4B_OK;
 }
 
+int make_tmap_pages(CUtensorMap* map, const q4b_paged_kv& kv, const void* base, uint32_t box_slots) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return set_error(Q4B_EUNSUPPORTED, "cuTensorMapEncodeTiled is not available from the driver");
+  // a dimension of one element may come with any stride: give it one that the map accepts
+  const cuuint64_t row = (cuuint64_t)kv.head_dim * 2;
+  auto stride = [&](int n, long long s) { return n > 1 ? (cuuint64_t)s * 2 : row; };
+  cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_kv_heads, (cuuint64_t)kv.n_pages};
+  cuuint64_t strides[3] = {stride(kv.page_size, kv.slot_stride), stride(kv.n_kv_heads, kv.head_stride),
+                           stride(kv.n_pages, kv.page_stride)};
+  cuuint32_t box[4] = {64, box_slots, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(Q4B_EINVAL, "cuTensorMapEncodeTiled (pages) failed (%d)", (int)r);
+  return Q4B_OK;
+}
+
 unsigned gemm_status(bool reset) {
   unsigned v = 0;
   cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(v));

@@ -126,7 +126,7 @@ __device__ Cursor cursor_at(int u, const PrefixArgs& a, const Shared& s) {
     c.b = -1;
     c.q0 = 0;
     c.n = a.rows;
-    c.len = a.b.prefix_len;
+    c.len = a.b.prefix_len - a.prefix_skip;
     c.row_tiles = (a.rows * a.g + kTileRows - 1) / kTileRows;
     c.tiles = (c.len + kTileKeys - 1) / kTileKeys;
   } else {
@@ -328,8 +328,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_attn_kernel(Pr
   sh.cum = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE);
   sh.q0 = sh.cum + a.b.batch + 1;
   sh.len = sh.q0 + a.b.batch + 1;
+  // Behind the tensor-core kernel the inputs are there already (it lets this kernel start only behind its own wait), and
+  // its results matter to the join alone, which must find both kernels complete: so the wait comes last.
   griddep_launch_dependents();
-  griddep_wait();
+  if (!a.tc_splits) griddep_wait();
 
   // the batch: rows, own keys and units of each sequence; thread t scans a run of sequences
   {
@@ -369,7 +371,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_attn_kernel(Pr
   }
   const int units = a.prefix_units + sh.cum[a.b.batch];
   const int ctas = min((int)gridDim.x, units);  // fewer units than CTAs: one each, so that no run is empty
-  if ((int)blockIdx.x >= ctas) return;
+  if ((int)blockIdx.x >= ctas) {
+    if (a.tc_splits) griddep_wait();
+    return;
+  }
   const int u0 = cta_first(blockIdx.x, units, ctas), u1 = cta_first(blockIdx.x + 1, units, ctas);
   const int count = u1 - u0;
 
@@ -380,9 +385,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_attn_kernel(Pr
   long long pend = -1;
   auto lookup = [&]() {
     if (tid < kTileKeys) {
-      const int key = look.tile * kTileKeys + tid;
+      int key = look.tile * kTileKeys + tid;
       pend = -1;
       if (key < look.limit) {
+        if (look.b < 0) key += a.prefix_skip;
         const int pi = key / a.kv.page_size;
         const int page = __ldg(look.b < 0 ? a.prefix_pages + pi : a.b.page_table + look.b * a.b.table_stride + pi);
         if (page >= 0 && page < a.kv.n_pages)
@@ -535,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_attn_kernel(Pr
       w.start(a, cur, split_keys ? 0 : warp * 16, lane);
     }
   }
+  if (a.tc_splits) griddep_wait();
 }
 
 // Joins a row's parts: one warp per (row, head). Every part is (max, sum, weighted V); the prefix's parts and the own
@@ -592,9 +599,18 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(PrefixArgs a, int grid
       }
     }
   };
+  const long long n_rows = (long long)a.rows * a.H;
+  for (int s = 0; s < a.tc_splits; s += 32) {
+    float2 x = make_float2(-INFINITY, 0.0f);
+    if (s + lane < a.tc_splits) x = __ldcg(a.tc_ml + (s + lane) * n_rows + row);
+    const int n = min(32, a.tc_splits - s);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k)
+      add(__shfl_sync(0xffffffffu, x.x, k), __shfl_sync(0xffffffffu, x.y, k), a.tc_o + ((s + k) * n_rows + row) * HD);
+  }
   if (a.prefix_units) {
     const int rr = t * a.g + head - h * a.g, rt = rr / kTileRows;
-    const int row_tiles = (a.rows * a.g + kTileRows - 1) / kTileRows, tiles = (a.b.prefix_len + kTileKeys - 1) / kTileKeys;
+    const int row_tiles = (a.rows * a.g + kTileRows - 1) / kTileRows, tiles = (a.b.prefix_len - a.prefix_skip + kTileKeys - 1) / kTileKeys;
     parts((h * row_tiles + rt) * tiles, tiles, rr - rt * kTileRows, a.row_o, a.row_ml);
   }
   const int mine = a.cum[b + 1] - a.cum[b];
@@ -624,18 +640,25 @@ int grid_of(int hd) { return hd == 128 ? ctas<128>() : hd == 64 ? ctas<64>() : c
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // workspace: cum | (max, sum) and weighted V by output row, prefix then own keys | the same of cut items
+// | the same of the tensor-core kernel's splits
 struct Plan {
-  size_t cum, row_ml, row_o, cut_ml, cut_o, total;
+  size_t cum, row_ml, row_o, cut_ml, cut_o, tc_ml, tc_o, total;
+  PrefixTcPlan tc;
 };
-Plan plan(int rows, int H, int hd, int batch) {
+Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv) {
   Plan p;
+  const int hd = kv.head_dim, batch = b.batch;
+  p.tc = prefix_tc_plan(rows, H, b.prefix_len, kv);
+  const size_t tc = (size_t)p.tc.splits * rows * H;
   const size_t n = 2 * (size_t)rows * H, cut = 2 * (size_t)grid_of(hd) * kTileRows;
   p.cum = 0;
   p.row_ml = up256((batch + 1) * sizeof(int));
   p.row_o = p.row_ml + up256(n * sizeof(float2));
   p.cut_ml = p.row_o + up256(n * hd * sizeof(float));
   p.cut_o = p.cut_ml + up256(cut * sizeof(float2));
-  p.total = p.cut_o + up256(cut * hd * sizeof(float));
+  p.tc_ml = p.cut_o + up256(cut * hd * sizeof(float));
+  p.tc_o = p.tc_ml + up256(tc * sizeof(float2));
+  p.total = p.tc_o + up256(tc * hd * sizeof(float));
   return p;
 }
 
@@ -679,7 +702,7 @@ using namespace q4b;
 
 extern "C" size_t q4b_prefix_attention_workspace(int rows, int n_heads, const q4b_batch* batch, const q4b_paged_kv* kv) {
   if (check("prefix_attention", rows, n_heads, batch, kv)) return 0;
-  return plan(rows, n_heads, kv->head_dim, batch->batch).total;
+  return plan(rows, n_heads, *batch, *kv).total;
 }
 
 extern "C" int q4b_prefix_attention(const void* q, long long q_stride, long long q_head_stride, int rows, int n_heads,
@@ -693,7 +716,7 @@ extern "C" int q4b_prefix_attention(const void* q, long long q_stride, long long
   if (q_stride % 2 || q_head_stride % 2 || !aligned(q, 4) || !aligned(out, 16))
     return set_error(Q4B_EINVAL, "%s: q must be 4-byte aligned with even strides, out 16-byte aligned", what);
   if (!(scale > 0.0f) || !(scale < INFINITY)) return set_error(Q4B_EINVAL, "%s: scale must be positive", what);
-  const Plan p = plan(rows, n_heads, kv->head_dim, batch->batch);
+  const Plan p = plan(rows, n_heads, *batch, *kv);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < p.total)
     return set_error(Q4B_EINVAL, "%s: needs a 256-byte aligned workspace of %zu bytes", what, p.total);
   PrefixArgs a;
@@ -701,14 +724,23 @@ extern "C" int q4b_prefix_attention(const void* q, long long q_stride, long long
   a.rows = rows, a.H = n_heads, a.Hkv = kv->n_kv_heads, a.g = n_heads / kv->n_kv_heads;
   a.scale2 = scale * 1.44269504088896340736f;
   a.b = *batch, a.kv = *kv, a.prefix_pages = prefix_pages, a.out = out;
-  a.prefix_units = a.Hkv * ((rows * a.g + kTileRows - 1) / kTileRows) * ((batch->prefix_len + kTileKeys - 1) / kTileKeys);
+  // the tensor-core kernel reads q in 16-byte pieces
+  const bool tc = p.tc.splits && aligned(q, 16) && q_stride % 8 == 0 && q_head_stride % 8 == 0;
+  a.tc_splits = tc ? p.tc.splits : 0, a.tc_pairs = p.tc.pairs, a.tc_tiles = p.tc.tiles;
+  a.prefix_skip = tc ? p.tc.tiles * 128 : 0;
+  a.prefix_units = a.Hkv * ((rows * a.g + kTileRows - 1) / kTileRows) *
+                   ((batch->prefix_len - a.prefix_skip + kTileKeys - 1) / kTileKeys);
   char* w = static_cast<char*>(workspace);
   a.cum = reinterpret_cast<int*>(w + p.cum);
   a.row_ml = reinterpret_cast<float2*>(w + p.row_ml);
   a.row_o = reinterpret_cast<float*>(w + p.row_o);
   a.cut_ml = reinterpret_cast<float2*>(w + p.cut_ml);
   a.cut_o = reinterpret_cast<float*>(w + p.cut_o);
+  a.tc_ml = reinterpret_cast<float2*>(w + p.tc_ml);
+  a.tc_o = reinterpret_cast<float*>(w + p.tc_o);
   const cudaStream_t st = as_stream(stream);
+  if (tc)
+    if (int rc = prefix_tc_run(a, st)) return rc;
   const bool h16 = kv->dtype == Q4B_F16;
   switch (kv->head_dim) {
     case 128: return h16 ? launch<__half, 128>(a, st) : launch<__nv_bfloat16, 128>(a, st);

@@ -136,5 +136,8 @@ int make_tmap_f16(CUtensorMap* map, const void* base, uint64_t cols, uint64_t ro
 // {box_cols, box_rows}; box_cols * 4 must be a multiple of 16 bytes.
 int make_tmap_i32(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t ld, uint32_t box_cols,
                   uint32_t box_rows);
+// 4-D map over a pool of pages (base: kv.k or kv.v), coordinates (element, slot, KV head, page); box {64
+// elements (128 B), box_slots, 1, 1}, 128-byte swizzle, pages out of the pool read as zero.
+int make_tmap_pages(CUtensorMap* map, const q4b_paged_kv& kv, const void* base, uint32_t box_slots);
 
 }  // namespace q4b

@@ -139,6 +139,14 @@ ATTEND = [
     ([(1, 1)] * 70, 16, 513, 8, 8, 128),  # more than one row tile of the prefix, one head per KV head
     ([(2, 2000)], 16, 3000, 8, 2, 128),
     ([(130, 130), (100, 700)], 16, 300, 4, 4, 32),
+    # prefixes of whole 128-key tiles and rests, for steps of more than 32 rows per KV head
+    ([(1, 5)] * 33, 16, 128, 2, 2, 64),
+    ([(1, 40)] * 50, 8, 1290, 8, 2, 64),
+    ([(3, 9), (40, 44)], 32, 127, 8, 2, 128),
+    ([(1, 1)] * 43, 64, 4096, 6, 2, 128),  # 129 rows: a second tile of one row
+    ([(70, 70), (60, 61)], 128, 640, 8, 4, 128),
+    ([(2, 2)] * 129, 256, 1000, 2, 1, 64),
+    ([(90, 100), (7, 300)], 512, 2200, 3, 1, 128),
 ]
 
 
@@ -205,6 +213,43 @@ def test_attend_leaves_padding_rows(q4b):
     assert got is out and live.tolist() == [True] * 3 + [False] * 3 and bool((out[3:] == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attend_bad_prefix_pages_hold_no_keys(q4b, hd, dtype):
+    """The same where the prefix runs in tiles: single pages, a whole tile and the first tile missing."""
+    case = _attend_case([(20, 70), (30, 40), (1, 8)], 16, 1000, 8, 4, hd, dtype, 5)
+    for i in list(range(8)) + [13] + list(range(24, 32)) + [40, 62]:
+        case[0]["prefix_pages"][i] = -1 if i % 2 else 2**31 - 1
+    _run_attend(q4b, case, 16)
+    case[0]["prefix_pages"][:] = 10**6
+    _run_attend(q4b, case, 16)
+
+
+def test_attend_growing_scores(q4b):
+    """Keys ordered by score, so that the running maximum grows from tile to tile, by little and by much."""
+    for step in (0.02, 2.0):
+        b, q, kp, vp = _attend_case([(1, 9)] * 40, 16, 1024, 4, 2, 64, torch.float16, 5)
+        q[:] = 0
+        q[:, :, 0] = 1.0
+        pages = torch.from_numpy(b["prefix_pages"]).long().to(DEV)
+        kp[pages, :, :, 0] = (torch.arange(1024, device=DEV).view(64, 16, 1) * step).half()
+        _run_attend(q4b, (b, q, kp, vp), 16, scale=0.4)
+
+
+def test_attend_prefix_tiles_from_other_orders(q4b):
+    """Head-major pages for the tiled prefix; and a q that the tiles cannot read in 16-byte pieces."""
+    b, q, kp, vp = _attend_case([(1, 30)] * 40, 16, 500, 8, 2, 64, torch.float16, 9)
+    both = torch.randn(kp.shape[0], 2, 2, 16, 64, device=DEV).half()
+    kp2, vp2 = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    kp2.copy_(kp), vp2.copy_(vp)
+    wide = torch.randn(40, 520, device=DEV).half()
+    q2 = wide[:, 2:514].view(40, 8, 64)
+    q2.copy_(q)
+    a, _, _ = _run_attend(q4b, (b, q, kp2, vp2), 16)
+    c, _, _ = _run_attend(q4b, (b, q2, kp2, vp2), 16)
+    assert float((a - c).abs().max()) < 0.01
+
+
 def test_attend_bad_pages_hold_no_keys(q4b):
     case = _attend_case([(1, 70), (3, 40), (1, 8)], 8, 100, 8, 2, 64, torch.float16, 5)
     case[0]["page_table"][0, 3], case[0]["page_table"][1, 4], case[0]["prefix_pages"][7] = -1, 10**6, 2**31 - 1
@@ -251,6 +296,7 @@ def test_attend_strides_scale_and_orders(q4b):
 def test_attend_sharp_scores(q4b):
     """Scores of some hundreds: the running maximum does the work."""
     _run_attend(q4b, _attend_case([(2, 300), (1, 31)], 16, 700, 8, 2, 64, torch.float16, 9, sharp=3.0), 16, scale=2.0)
+    _run_attend(q4b, _attend_case([(20, 300), (10, 31)], 16, 700, 8, 2, 64, torch.float16, 9, sharp=3.0), 16, scale=2.0)
 
 
 def test_attend_far_pages(q4b):
