@@ -35,15 +35,17 @@ __device__ __forceinline__ int2 batch_rows(const int32_t* q_start, int b, int ro
   return make_int2(lo, min(max(__ldg(q_start + b + 1), lo), rows));
 }
 
-// The sequence that holds row t, or -1: the last b with q_start[b] <= t, if its rows reach t.
-__device__ __forceinline__ int batch_find(const int32_t* q_start, int batch, int t) {
-  int lo = 0, hi = batch;  // first b in [0, batch] with q_start[b] > t
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(q_start + mid) <= t)
-      lo = mid + 1;
-    else
-      hi = mid;
+// The sequence that holds row t, or -1: the last b with q_start[b] <= t, if its rows reach t. By a whole warp, 32
+// probes a round: the loads of a round run side by side (one round up to 32 sequences, two up to 1055).
+__device__ __forceinline__ int batch_find(const int32_t* q_start, int batch, int t, int lane) {
+  int lo = 0, n = batch;  // the first b with q_start[b] > t is in [lo, lo + n]
+  while (n > 0) {
+    const int step = (n + 31) / 32, at = lane * step;
+    const int c = __popc(__ballot_sync(0xffffffffu, at < n && __ldg(q_start + lo + min(at, n - 1)) <= t));
+    if (c == 0) break;
+    const int skip = (c - 1) * step + 1;
+    lo += skip;
+    n = min(step - 1, n - skip);
   }
   if (lo == 0) return -1;
   return t < __ldg(q_start + lo) ? lo - 1 : -1;

@@ -7,9 +7,8 @@
 // Bound by memory: every element is read once and written once (plus 4 rot bytes of table per token, read
 // through L1 by the token's heads). A task is 16 elements of one head: both sides of eight pairs, so that
 // every access is 16 or 32 bytes. A CTA takes `tok` tokens: first each token's place (sequence, page, slot,
-// position) is found by one thread, with the binary searches of all its tokens running side by side, then
-// all threads walk the tasks. Few tokens get one CTA each (latency), many share CTAs so that the
-// searches are paid once per 8 tokens.
+// position) is found by one warp, then all threads walk the tasks. Few tokens get one CTA each (latency),
+// many share CTAs so that the searches are paid once per 8 tokens.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -44,7 +43,7 @@ int check_paged_kv(const char* what, const q4b_paged_kv* kv) {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kMaxTok = 8;
+constexpr int kMaxTok = kAppendThreads / 32;
 
 struct AppendArgs {
   const void *q, *k, *v;
@@ -95,9 +94,10 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
   const int t0 = blockIdx.x * a.tok, nt = min(a.tok, a.rows - t0);
   griddep_launch_dependents();
   griddep_wait();
-  if (threadIdx.x < nt) {
-    const int t = t0 + threadIdx.x;
-    const int b = batch_find(a.b.q_start, a.b.batch, t);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < nt) {
+    const int t = t0 + warp;
+    const int b = batch_find(a.b.q_start, a.b.batch, t, lane);
     int state = kSkip;
     long long off = -1, pos = 0;
     if (b >= 0) {
@@ -114,9 +114,11 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
           off = page * a.kv.page_stride + (s - (long long)pi * a.kv.page_size) * a.kv.slot_stride;
       }
     }
-    s_state[threadIdx.x] = state;
-    s_off[threadIdx.x] = off;
-    s_pos[threadIdx.x] = pos;
+    if (lane == 0) {
+      s_state[warp] = state;
+      s_off[warp] = off;
+      s_pos[warp] = pos;
+    }
   }
   __syncthreads();
 

@@ -544,91 +544,109 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_attn_kernel(Pr
   if (a.tc_splits) griddep_wait();
 }
 
-// Joins a row's parts: one warp per (row, head). Every part is (max, sum, weighted V); the prefix's parts and the own
-// keys' come from whichever CTAs' runs the row's items lie in.
+// Joins a row's parts, a warp per (row, head): every part is (max, sum, weighted V); the prefix's and the own keys'
+// come from whichever CTAs' runs the row's items lie in, 32 parts a round with all their loads side by side.
+// Bound by latency (batch search, (max, sum), V: three dependent loads) until the parts outgrow L2; `per`
+// rows a warp keep the grid to one wave.
+constexpr int kJoinWarps = 4, kJoinResident = kSms * 48;  // warps that run at once
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) prefix_join_kernel(PrefixArgs a, int grid) {
+__global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(PrefixArgs a, int grid, int per) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const long long n_rows = (long long)a.rows * a.H;
+  const long long row0 = ((long long)blockIdx.x * kJoinWarps + (threadIdx.x >> 5)) * per;
   griddep_launch_dependents();
   griddep_wait();
-  if (row >= (long long)a.rows * a.H) return;
-  const int t = (int)(row / a.H), head = (int)(row - (long long)t * a.H), h = head / a.g;
-  const int b = batch_find(a.b.q_start, a.b.batch, t);
-  if (b < 0) return;
-  const int units = a.prefix_units + a.cum[a.b.batch], ctas = min(grid, units);
-  float acc[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-
-  auto add = [&](float m2, float l2, const float* o) {  // uniform over the warp
-    if (l2 == 0.0f && m2 == -INFINITY) return;
-    const float mm = fmaxf(m, m2), f = exp2f(m - mm), f2 = exp2f(m2 - mm);
-    float v[E];
-    if constexpr (E == 4) {
-      *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(o) + lane);
-    } else if constexpr (E == 2) {
-      *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(o) + lane);
-    } else {
-      v[0] = __ldcg(o + lane);
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(v[e], f2, acc[e] * f);
-    l = fmaf(l2, f2, l * f);
-    m = mm;
-  };
-  // parts of the item with units [first, first + tiles), at row r of its row tile
-  auto parts = [&](int first, int tiles, int r, const float* row_o, const float2* row_ml) {
-    const int c0 = cta_of(first, units, ctas), c1 = cta_of(first + tiles - 1, units, ctas);
-    if (c0 == c1) {
-      const float2 x = __ldcg(row_ml + row);
-      add(x.x, x.y, row_o + row * HD);
-      return;
-    }
-    for (int c = c0; c <= c1; c += 32) {
-      const int mine = c + lane;
-      const int at = (2 * mine + (mine == c0)) * kTileRows + r;
-      float2 x = make_float2(-INFINITY, 0.0f);
-      if (mine <= c1) x = __ldcg(a.cut_ml + at);
-      const int n = min(32, c1 - c + 1);
-#pragma unroll 4
-      for (int k = 0; k < n; ++k) {
-        const int from = (2 * (c + k) + (c + k == c0)) * kTileRows + r;
-        add(__shfl_sync(0xffffffffu, x.x, k), __shfl_sync(0xffffffffu, x.y, k), a.cut_o + (long long)from * HD);
+  const int units = a.prefix_units + __ldcg(a.cum + a.b.batch), ctas = min(grid, units);
+  const int p_row_tiles = (a.rows * a.g + kTileRows - 1) / kTileRows;
+  const int p_tiles = (a.b.prefix_len - a.prefix_skip + kTileKeys - 1) / kTileKeys;
+  int t = -1, b = -1, q0 = 0, own_first = 0, own_row_tiles = 1, own_tiles = 0;
+  for (long long row = row0; row < min(row0 + per, n_rows); ++row) {
+    const int head = (int)(row % a.H), h = head / a.g;
+    if ((int)(row / a.H) != t) {
+      t = (int)(row / a.H);
+      b = batch_find(a.b.q_start, a.b.batch, t, lane);
+      if (b >= 0) {
+        const int2 r = batch_rows(a.b.q_start, b, a.rows);
+        const int c0 = __ldcg(a.cum + b), c1 = __ldcg(a.cum + b + 1);
+        q0 = r.x;
+        own_first = a.prefix_units + c0;
+        own_row_tiles = ((r.y - r.x) * a.g + kTileRows - 1) / kTileRows;
+        own_tiles = (c1 - c0) / (max(own_row_tiles, 1) * a.Hkv);
       }
     }
-  };
-  const long long n_rows = (long long)a.rows * a.H;
-  for (int s = 0; s < a.tc_splits; s += 32) {
-    float2 x = make_float2(-INFINITY, 0.0f);
-    if (s + lane < a.tc_splits) x = __ldcg(a.tc_ml + (s + lane) * n_rows + row);
-    const int n = min(32, a.tc_splits - s);
+    if (b < 0) continue;
+    // the prefix's item and the own keys' item of this row: its row in the row tile, first CTA, number of parts
+    const int pr = t * a.g + head - h * a.g, orow = (t - q0) * a.g + head - h * a.g;
+    int p_c0 = 0, p_n = 0, o_c0 = 0, o_n = 0;
+    if (p_tiles > 0) {
+      const int u = (h * p_row_tiles + pr / kTileRows) * p_tiles;
+      p_c0 = cta_of(u, units, ctas);
+      p_n = cta_of(u + p_tiles - 1, units, ctas) - p_c0 + 1;
+    }
+    if (own_tiles > 0) {
+      const int u = own_first + (h * own_row_tiles + orow / kTileRows) * own_tiles;
+      o_c0 = cta_of(u, units, ctas);
+      o_n = cta_of(u + own_tiles - 1, units, ctas) - o_c0 + 1;
+    }
+    const int parts = a.tc_splits + p_n + o_n;
+    float acc[E], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      int k = k0 + lane;
+      float2 x = make_float2(-INFINITY, 0.0f);
+      const float* o = a.row_o;
+      if (k < a.tc_splits) {
+        x = __ldcg(a.tc_ml + k * n_rows + row);
+        o = a.tc_o + (k * n_rows + row) * HD;
+      } else if (k < parts) {
+        k -= a.tc_splits;
+        const bool pre = k < p_n;
+        if (!pre) k -= p_n;
+        if ((pre ? p_n : o_n) == 1) {
+          const long long at = row + (pre ? 0 : n_rows);
+          x = __ldcg(a.row_ml + at);
+          o = a.row_o + at * HD;
+        } else {
+          const int at = (2 * ((pre ? p_c0 : o_c0) + k) + (k == 0)) * kTileRows + (pre ? pr : orow) % kTileRows;
+          x = __ldcg(a.cut_ml + at);
+          o = a.cut_o + (long long)at * HD;
+        }
+      }
+      const float mm = fmaxf(m, warp_max(x.x)), ref = mm == -INFINITY ? 0.0f : mm;
+      const float f = exp2f(m - ref), weight = exp2f(x.x - ref);  // a part without keys: 0
+      l = l * f + warp_sum(x.y * weight);
+      m = mm;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= f;
+      const int n = min(32, parts - k0);
 #pragma unroll 4
-    for (int k = 0; k < n; ++k)
-      add(__shfl_sync(0xffffffffu, x.x, k), __shfl_sync(0xffffffffu, x.y, k), a.tc_o + ((s + k) * n_rows + row) * HD);
+      for (int i = 0; i < n; ++i) {
+        const float w = __shfl_sync(0xffffffffu, weight, i);
+        const float* src = reinterpret_cast<const float*>(
+            __shfl_sync(0xffffffffu, (unsigned long long)reinterpret_cast<uintptr_t>(o), i)) + lane * E;
+        float v[E];
+        if constexpr (E == 4)
+          *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(src));
+        else if constexpr (E == 2)
+          *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(src));
+        else
+          v[0] = __ldcg(src);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(v[e], w, acc[e]);
+      }
+    }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no keys: zero
+    T* out = static_cast<T*>(a.out) + row * HD + lane * E;
+    if constexpr (E == 4)
+      *reinterpret_cast<uint2*>(out) = make_uint2(Half16<T>::pack(acc[0] * inv, acc[1] * inv), Half16<T>::pack(acc[2] * inv, acc[3] * inv));
+    else if constexpr (E == 2)
+      *reinterpret_cast<uint32_t*>(out) = Half16<T>::pack(acc[0] * inv, acc[1] * inv);
+    else
+      *out = T(acc[0] * inv);
   }
-  if (a.prefix_units) {
-    const int rr = t * a.g + head - h * a.g, rt = rr / kTileRows;
-    const int row_tiles = (a.rows * a.g + kTileRows - 1) / kTileRows, tiles = (a.b.prefix_len - a.prefix_skip + kTileKeys - 1) / kTileKeys;
-    parts((h * row_tiles + rt) * tiles, tiles, rr - rt * kTileRows, a.row_o, a.row_ml);
-  }
-  const int mine = a.cum[b + 1] - a.cum[b];
-  if (mine) {
-    const int2 r = batch_rows(a.b.q_start, b, a.rows);
-    const int rr = (t - r.x) * a.g + head - h * a.g, rt = rr / kTileRows;
-    const int row_tiles = ((r.y - r.x) * a.g + kTileRows - 1) / kTileRows, tiles = mine / (row_tiles * a.Hkv);
-    parts(a.prefix_units + a.cum[b] + (h * row_tiles + rt) * tiles, tiles, rr - rt * kTileRows,
-          a.row_o + (long long)a.rows * a.H * HD, a.row_ml + (long long)a.rows * a.H);
-  }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no keys: zero
-  T* out = static_cast<T*>(a.out) + row * HD + lane * E;
-  if constexpr (E == 4)
-    *reinterpret_cast<uint2*>(out) = make_uint2(Half16<T>::pack(acc[0] * inv, acc[1] * inv), Half16<T>::pack(acc[2] * inv, acc[3] * inv));
-  else if constexpr (E == 2)
-    *reinterpret_cast<uint32_t*>(out) = Half16<T>::pack(acc[0] * inv, acc[1] * inv);
-  else
-    *out = T(acc[0] * inv);
 }
 
 template <int HD>
@@ -670,8 +688,11 @@ int launch(const PrefixArgs& a, cudaStream_t st) {
   cudaError_t e = set_max_dynamic_smem(kern, C::STAGES * C::STAGE + 12 * (kMaxBatch + 1), done);
   if (e == cudaSuccess)
     e = launch_pdl(kern, dim3(ctas<HD>()), dim3(kThreads), C::STAGES * C::STAGE + 12 * (a.b.batch + 1), st, a);
+  const long long n = (long long)a.rows * a.H;
+  const int per = (int)((n + kJoinResident - 1) / kJoinResident);
   if (e == cudaSuccess)
-    e = launch_pdl(prefix_join_kernel<T, HD>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4)), dim3(128), 0, st, a, ctas<HD>());
+    e = launch_pdl(prefix_join_kernel<T, HD>, dim3((unsigned)((n + kJoinWarps * per - 1) / (kJoinWarps * per))),
+                   dim3(32 * kJoinWarps), 0, st, a, ctas<HD>(), per);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(Q4B_ELAUNCH, "prefix_attention: launch failed: %s", cudaGetErrorString(e));

@@ -5,9 +5,9 @@
 //   w = max(p - d, 0) of that row (p of the last row if all were kept): the first j with W_j > u W_{V-1}, W the
 //   running sum of w.
 //
-// The sums are in 64 bits: a running sum of 10^5 probabilities in fp32 is off by more than a typical w, and the
-// drawn index would depend on the order of the sum. u d and p - d of two fp32 (or shorter) numbers are exact in
-// 64 bits (p - d up to an exponent difference of 29, beyond which the error is below 2^-53 p).
+// The sums have 43 bits and more (64-bit words where it matters, pairs of fp32 words over the values of a
+// lane): a running sum of 10^5 probabilities in fp32 is off by more than a typical w, and the
+// drawn index would depend on the order of the sum. The products u d of the tests are exact in 64 bits.
 //
 // Bound by memory: one row of p, and of d where a draft was rejected, per sequence; the acceptance tests read
 // two numbers per draft. A cluster of CTAs takes one sequence, so that a row's read is spread over several
@@ -62,33 +62,82 @@ struct Weights {
 template <typename T, int N>
 __device__ __forceinline__ void unpack16(const uint4& v, float (&x)[N]) {
   static_assert(N == 16 / sizeof(T), "one 16-byte vector");
-  const T* e = reinterpret_cast<const T*>(&v);
+  if constexpr (sizeof(T) == 4) {
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+  } else {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = as_float(e[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Half16<T>::unpack(u[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
 }
 
-// Sum of the weights of [lo, lo + kTile), a tile whose bounds are 16-byte aligned in p and d, by one warp;
-// every lane gets it.
+// A sum in two fp32 words. The error of each fp32 addition and subtraction is itself an fp32 number, found
+// by Knuth's two-sum; the errors are added up in `lo`. Over the 32 values of a lane hi + lo is off by
+// less than 2^-43 of the sum, far below the share of one token, at fp32 speed: conversions to 64
+// bits and 64-bit additions for every value took three times as long as the row's read.
+struct Sum2 {
+  float hi = 0.0f, lo = 0.0f;
+  float top = 0.0f;  // largest value met: an infinite one sends the tile to the careful sum
+  __device__ __forceinline__ void add(float x, float e) {
+    const float s = __fadd_rn(hi, x), b = __fsub_rn(s, hi);
+    lo = __fadd_rn(lo, __fadd_rn(__fadd_rn(__fsub_rn(hi, __fsub_rn(s, b)), __fsub_rn(x, b)), e));
+    hi = s;
+  }
+  __device__ __forceinline__ void add_target(float p) {
+    p = fmaxf(p, 0.0f);  // NaN and negative: zero
+    top = fmaxf(top, p);
+    add(p, 0.0f);
+  }
+  __device__ __forceinline__ void add_rest(float p, float d) {
+    p = fmaxf(p, 0.0f), d = fmaxf(d, 0.0f);
+    top = fmaxf(top, fmaxf(p, d));
+    const float s = __fsub_rn(p, d), b = __fsub_rn(s, p);
+    const float e = __fsub_rn(__fsub_rn(p, __fsub_rn(s, b)), __fadd_rn(d, b));
+    if (s > 0.0f) add(s, e);  // the rounded difference has the exact one's sign
+  }
+};
+
+// This lane's share of the weights of tile [lo, lo + kTile), whose bounds are 16-byte aligned in p and d: every
+// 32nd vector (coalesced), or, with `runs`, the 32 values from lo + 32 lane.
 template <typename T>
-__device__ __forceinline__ double tile_sum_vec(const Weights<T>& w, int lo, int lane) {
-  constexpr int N = 16 / sizeof(T), U = kTile / (32 * N);
-  uint4 pv[U], dv[U];
+__device__ __forceinline__ double lane_sum_vec(const Weights<T>& w, int lo, int lane, bool runs) {
+  constexpr int N = 16 / sizeof(T), U = kTile / (32 * N), HALF = U / 2;
+  Sum2 sum;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    pv[u] = ld_stream_u4(w.p + lo + (u * 32 + lane) * N);
-    dv[u] = w.d ? ld_stream_u4(w.d + lo + (u * 32 + lane) * N) : make_uint4(0, 0, 0, 0);
+  for (int h = 0; h < 2; ++h) {
+    uint4 pv[HALF], dv[HALF];
+    auto first = [&](int u) { return lo + N * (runs ? lane * U + h * HALF + u : (h * HALF + u) * 32 + lane); };
+#pragma unroll
+    for (int u = 0; u < HALF; ++u) {
+      pv[u] = ld_stream_u4(w.p + first(u));
+      if (w.d) dv[u] = ld_stream_u4(w.d + first(u));
+    }
+#pragma unroll
+    for (int u = 0; u < HALF; ++u) {
+      float a[N];
+      unpack16<T>(pv[u], a);
+      if (w.d) {
+        float b[N];
+        unpack16<T>(dv[u], b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum.add_rest(a[i], b[i]);
+      } else {
+        const unsigned at = (unsigned)(w.skip - first(u));
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum.add_target(at == (unsigned)i ? 0.0f : a[i]);
+      }
+    }
   }
-  double s = 0.0;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    float a[N], b[N];
-    unpack16<T>(pv[u], a);
-    unpack16<T>(dv[u], b);
-    const int i0 = lo + (u * 32 + lane) * N;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s += i0 + i == w.skip ? 0.0 : w.of(a[i], b[i]);
+  const bool odd = !(sum.top < INFINITY && sum.hi < INFINITY);
+  if (__any_sync(0xffffffffu, odd)) {  // an infinite value counts as zero
+    double s = 0.0;
+    for (int i = 0; i < kTile / 32; ++i) s += w.at(lo + (runs ? lane * (kTile / 32) + i : i * 32 + lane));
+    return s;
   }
-  return s;
+  return (double)sum.hi + (double)sum.lo;
 }
 
 template <typename T>
@@ -116,7 +165,7 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads) verify_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kVfThreads, 4) verify_kernel(VerifyArgs a) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -185,7 +234,7 @@ __global__ void __launch_bounds__(kVfThreads) verify_kernel(VerifyArgs a) {
     double mine = 0.0;
     for (int t = t_lo + warp; t < t_hi; t += kVfWarps) {
       const int lo = lo_of(t), hi = hi_of(t);
-      const double s = warp_sum(vec && hi - lo == kTile ? tile_sum_vec(w, lo, lane) : tile_sum_any(w, lo, hi, lane));
+      const double s = warp_sum(vec && hi - lo == kTile ? lane_sum_vec(w, lo, lane, false) : tile_sum_any(w, lo, hi, lane));
       if (lane == 0) s_tile[t - t_lo] = s;
       mine += s;
     }
@@ -251,27 +300,26 @@ __global__ void __launch_bounds__(kVfThreads) verify_kernel(VerifyArgs a) {
   }
   if (tile < 0) tile = tile_some;
 
-  // its index: lane l holds a run of the tile's values
+  // its run of values: lane l sums run l of the tile
   const int lo = lo_of(tile), hi = hi_of(tile), per = (hi - lo + 31) / 32;
   const int from = min(lo + lane * per, hi), to = min(from + per, hi);
   double s = 0.0;
+  if (hi - lo == kTile && (!w.d || reinterpret_cast<uintptr_t>(w.d) % 16 == reinterpret_cast<uintptr_t>(w.p) % 16)) {
+    s = lane_sum_vec(w, lo, lane, true);
+  } else {
 #pragma unroll 8
-  for (int i = from; i < to; ++i) s += w.at(i);
-  const double end = tile_base + warp_scan(s, lane);
-  const unsigned above = __ballot_sync(0xffffffffu, s > 0.0 && end > mark), any = __ballot_sync(0xffffffffu, s > 0.0);
-  const int f = above ? __ffs(above) - 1 : 31 - __clz(any);
-  if (lane != f) return;
-  double at = end - s;
-  int pick = -1;
-  for (int i = from; i < to; ++i) {
-    const double v = w.at(i);
-    if (v > 0.0) {
-      pick = i;
-      at += v;
-      if (at > mark) break;
-    }
+    for (int i = from; i < to; ++i) s += w.at(i);
   }
-  a.out_tokens[row] = pick;
+  double end = tile_base + warp_scan(s, lane);
+  unsigned above = __ballot_sync(0xffffffffu, s > 0.0 && end > mark), any = __ballot_sync(0xffffffffu, s > 0.0);
+  const int f = above ? __ffs(above) - 1 : 31 - __clz(any);
+  // its value: lane l takes value l of the run
+  const int i = __shfl_sync(0xffffffffu, from, f) + lane;
+  const double run_base = __shfl_sync(0xffffffffu, end - s, f);
+  s = i < __shfl_sync(0xffffffffu, to, f) ? w.at(i) : 0.0;
+  end = run_base + warp_scan(s, lane);
+  above = __ballot_sync(0xffffffffu, s > 0.0 && end > mark), any = __ballot_sync(0xffffffffu, s > 0.0);
+  if (lane == (above ? __ffs(above) - 1 : 31 - __clz(any))) a.out_tokens[row] = i;
 }
 
 template <typename T>
