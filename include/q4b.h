@@ -257,7 +257,7 @@ int q4b_prefix_attention(const void* q, long long q_stride, long long q_head_str
  *   uniforms[r] * draft[r, x] < target[r, x],  x = tokens[r + 1];
  * behind the n_b kept ones a token is drawn from max(target - draft, 0) of row q_start[b] + n_b (draft NULL:
  * target without x; a residual of zero: target), or, with every draft kept, from the last row's target: the first index whose running
- * sum exceeds uniforms[last row] * sum. Sums carry 43 bits and more. Probabilities that are negative or not finite
+ * sum exceeds uniforms[last row] * sum. Sums carry 40 bits and more. Probabilities that are negative or not finite
  * count as zero, a draft outside [0, vocab) is not kept, and weights that are all zero give the token -1.
  * out_tokens [rows]: at b's rows the kept drafts, the drawn token, then -1; accepted [batch] = n_b (0 for a
  * sequence without rows). dtype of target and draft: Q4B_F32, Q4B_F16 or Q4B_BF16; rows target_stride /

@@ -5,6 +5,13 @@
 
 namespace q4b {
 
+// The work of one kernel: items (KV head, row tile) of the prefix and of the sequences whose rows times heads per KV head
+// lie in (own_lo, own_hi], all their key tiles ("units") in one line, of which each CTA takes an equal run.
+struct AttnLine {
+  int prefix_units;
+  int own_lo, own_hi;
+};
+
 struct PrefixArgs {
   const void* q;  // [rows, H, hd] of the cache's type
   long long q_stride, q_head_stride;
@@ -14,25 +21,28 @@ struct PrefixArgs {
   q4b_paged_kv kv;
   const int32_t* prefix_pages;
   void* out;  // [rows, H * hd]
-  int prefix_units;  // key tiles of the prefix's items
-  int* cum;          // [batch + 1] key tiles of the own keys' items in front of sequence b
-  float2* row_ml;    // [2][rows * H] (max, sum) of whole items, prefix then own keys
+  int tc_ctas;       // CTAs of the tensor-core kernel, 0: not launched
+  int mm_ctas;       // CTAs of the mma.sync kernel
+  int mm_rows;       // its rows per row tile
+  AttnLine tc, mm;
+  int4* rec;         // [rows]: where the join finds a row's own item (see RowRec)
+  int* totals;       // units of the mm line, own units of the tc line
+  float2* row_ml;    // [2][rows * H] (max, sum) of items that one CTA did whole, prefix then own keys
   float* row_o;      // [2][rows * H][hd] their weighted V
-  float2* cut_ml;    // [CTAs][2][row tile] the same of cut items
-  float* cut_o;
-  // the prefix's whole 128-key tiles on the tensor cores (tc_splits 0: not used); the rest of the prefix, from key
-  // prefix_skip, stays with the other kernel
-  int tc_splits, tc_pairs, tc_tiles, prefix_skip;
-  float2* tc_ml;  // [tc_splits][rows * H]
-  float* tc_o;    // [tc_splits][rows * H][hd]
+  float2* mm_ml;     // [CTAs][2][mm_rows] the same of items cut between CTAs
+  float* mm_o;
+  float2* tc_ml;     // [prefix, own][CTAs][2][kTcRows]
+  float* tc_o;
 };
 
-struct PrefixTcPlan {
-  int splits, pairs, tiles;  // splits 0: the tensor-core kernel does not take this call
-};
-constexpr int kTcMaxSplits = 32;
-constexpr int kTcMinRows = 33;
-PrefixTcPlan prefix_tc_plan(int rows, int H, int prefix_len, const q4b_paged_kv& kv);
+constexpr int kTcRows = 256, kTcKeys = 128, kTcCtas = 148;
+constexpr int kMmKeys = 64;
+constexpr int kTcMaxBatch = 2048;  // the sequences' table shares the tensor-core kernel's shared memory
+constexpr int kTcMinUnits = 5000;  // prefix tiles of 16 rows x 64 keys from which the tensor-core kernel pays off
+constexpr int kTcMinRows = 64;     // rows x heads of a sequence from which it takes the own keys
+
+// whether the tensor-core kernel can read this cache
+bool prefix_tc_takes(const q4b_paged_kv& kv);
 int prefix_tc_run(const PrefixArgs& a, cudaStream_t st);
 unsigned prefix_status(bool reset);
 

@@ -1,33 +1,40 @@
-// The shared prefix's part of the batched attention on the tcgen05 tensor cores, for steps whose rows fill
-// them: all rows of the step and all heads of a KV head's group attend to the same keys, so QK and PV are
-// matrix products with M = rows * H / n_kv_heads.
+// Batched attention on the tcgen05 tensor cores, for the items with many rows: the shared prefix, where all
+// rows of the step and all heads of a KV head's group attend to the same keys, and the sequences with many
+// new rows. QK and PV are then matrix products with M = rows * heads per KV head.
 //
 //   S = Q K^T * scale;  P = exp2(S log2e - m);  O += P V;  l += sum P       (m: a running reference per row)
 //
-// One CTA per SM takes 256 query rows (two tiles of 128) of one KV head and a run of 128-key tiles; a row
-// tile's keys are split over several CTAs so that the CTAs fill the SMs, and each leaves (m, l) and O in
-// fp32 for the join kernel. Warps 0-3 and 4-7 are the softmax of one query tile each, a thread a row; warp 8
-// brings K and V tiles by TMA (a box per page, 128-byte swizzle, a ring of tiles); one thread of warp 9 issues
-// the MMAs. S and O live in TMEM (2 x 128 + 2 x head_dim columns), and P goes back into S's
-// columns as the A operand of the PV product, so nothing but K, V and Q passes through shared memory. The
-// two query tiles alternate: while one's softmax runs, the tensor core works for the other, and both use every
-// K and V tile that comes in.
+// One CTA per SM takes an equal run of the prefix's items and one of the own keys' (attn_line.cuh; row tiles of 256,
+// key tiles of 128).
+// Warps 0-3 and 4-7 are the softmax of one half of the row tile each, a thread a row; warp 8 brings K and V tiles by TMA
+// (a box per page, 128-byte swizzle, a ring of tiles that runs on across items); one thread of warp 9 issues the
+// MMAs (two more warps only fill up the warpgroup that gives up registers). S and O live in TMEM (2 x 128 + 2 x head_dim columns), and P goes back into S's columns as the A
+// operand of the PV product, so nothing but K, V and Q passes through shared memory. The two halves alternate: while
+// one's softmax runs, the tensor core works for the other, and both use every K and V tile that comes in. The
+// next item's Q and first product overlap the end of the item before.
 //
 // m moves only when a row's maximum outgrows it by 2^8, which keeps P below 256 and spares most tiles the pass over
 // O; exactness is not affected (l and O carry the same factor). P is rounded to the cache's type, as in
-// the other kernel. Bound by the tensor pipe and the exponentials (16 a clock per SM: 256 x 128 of them take as
-// long as the tile's two MMAs at their nominal rate).
+// the other kernel. Masks (the end of the keys, causal rows, pages that do not exist) cost only where a tile has
+// any: scores by selection, and V by zeros written over the tile where some row may not see a key, since
+// 0 * V is not 0 for infinite or NaN V; what such a V gives to the rows that do see it is added at the end.
+//
+// Bound by the tensor pipe and the exponentials (16 a clock per SM: 256 x 128 of them take as long as the
+// tile's two MMAs at their nominal rate).
 #include <type_traits>
 
-#include "paged.cuh"
-#include "prefix_attn.h"
+#include "attn_line.cuh"
 #include "tc.cuh"
 
 namespace q4b {
 namespace {
 
-constexpr int kTcThreads = 320;
-constexpr int kTcRows = 128, kTcKeys = 128;
+constexpr int kTcThreads = 384;
+// Registers: the softmax groups (256 threads) take from the four other warps; together no more than the 168
+// a thread that the block is launched with (256 * 208 + 128 * 80 <= 384 * 168).
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 80;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kTcThreads * kRegsLaunch, "setmaxnreg draws on the block's own registers");
+constexpr int kHalf = kTcRows / 2;  // rows of one softmax group and MMA
 constexpr float kSlack = 8.0f;  // base-2 growth of a row's maximum that its reference tolerates
 
 __device__ unsigned g_prefix_status = 0;
@@ -36,8 +43,8 @@ template <int HD>
 struct TcCfg {
   static constexpr int HALVES = HD / 64;                   // 64-column (128-byte) halves of a row
   static constexpr int ATOM = kTcKeys * 128;               // one half of a 128-row tile, bytes
-  static constexpr int TILE = HALVES * ATOM;               // Q, K or V tile
-  static constexpr int SLOTS = HD == 128 ? 5 : 8;          // K and V tiles in flight
+  static constexpr int TILE = HALVES * ATOM;               // Q half, K or V tile
+  static constexpr int SLOTS = HD == 128 ? 4 : 8;          // K and V tiles in flight
   static constexpr int SMEM = (2 + SLOTS) * TILE + 1024;   // + alignment to the swizzle's 1024 bytes
 };
 
@@ -89,12 +96,83 @@ __device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t (&r)[3
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// 32 bytes, one whole sector, of one row
+__device__ __forceinline__ void st_8(float* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// The run of one item that a CTA takes: tiles [t0, t1) of the cursor's item, of which those from `e1` on hold no key
+// that a row of it sees.
+struct Seg {
+  Cursor c;
+  int t0, t1, e1;
+  __device__ __forceinline__ int n() const { return max(e1 - t0, 0); }
+  __device__ __forceinline__ int active() const { return c.nrows > kHalf ? 2 : 1; }
+};
+
+// The segments of a CTA's runs, in order: one run of the own keys' units and one of the prefix's. Each is an equal share,
+// so that the two kinds, whose units cost differently, spread evenly.
+struct Segs {
+  const Line<kTcRows, kTcKeys>& line;
+  int u, u1, then0, then1;
+  Seg s;
+  __device__ __forceinline__ Segs(const Line<kTcRows, kTcKeys>& line, int2 own, int2 prefix)
+      : line(line), u(own.x), u1(own.y), then0(prefix.x), then1(prefix.y) {
+    start();
+  }
+  __device__ __forceinline__ void start() {
+    if (u >= u1) {
+      u = then0, u1 = then1;
+      then0 = then1 = 0;
+    }
+    if (u < u1) {
+      s.c = line.at(u);
+      set();
+    }
+  }
+  __device__ __forceinline__ void set() {
+    s.t0 = s.c.tile;
+    s.t1 = min(s.c.tiles, s.t0 + u1 - u);
+    s.e1 = min(s.t1, (s.c.limit + kTcKeys - 1) / kTcKeys);
+  }
+  __device__ __forceinline__ bool valid() const { return u < u1; }
+  __device__ __forceinline__ void next() {
+    u += s.t1 - s.t0;
+    if (u < u1) {
+      line.next_item(s.c);
+      set();
+    } else {
+      start();
+    }
+  }
+};
+
+__device__ __forceinline__ const int32_t* page_row(const PrefixArgs& a, const Cursor& c) {
+  return c.b < 0 ? a.prefix_pages : a.b.page_table + c.b * a.b.table_stride;
+}
+
+// The top bit of each half of the result: whether that half of v is an infinity or NaN (exponent all ones).
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t v) {
+  constexpr bool H16 = std::is_same<T, __half>::value;
+  return (v & (H16 ? 0x7C007C00u : 0x7F807F80u)) + (H16 ? 0x04000400u : 0x00800080u);
 }
 
 template <typename T, int HD>
@@ -104,33 +182,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
-  __shared__ uint64_t full[C::SLOTS], empty[C::SLOTS], q_full, s_full[2], p_full[2], o_full[2], drained;
+  __shared__ uint64_t full[C::SLOTS], empty[C::SLOTS], q_full[2], s_full[2], p_full[2], o_full[2], drained;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_fail, s_issued;
-  constexpr uint32_t kS = 0, kO = 256;  // TMEM columns: S (and P) of tile i at 128 i, O at 256 + HD i
+  __shared__ int s_fail, s_issued, s_odd, s_scan[kTcThreads / 32];
+  constexpr uint32_t kS = 0, kO = 256;  // TMEM columns: S (and P) of half i at 128 i, O at 256 + HD i
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // item: KV head, pair of row tiles, run of key tiles
-  const int sp = blockIdx.x % a.tc_splits, pair = blockIdx.x / a.tc_splits % a.tc_pairs,
-            h = blockIdx.x / a.tc_splits / a.tc_pairs;
-  const int j0 = (int)((long long)sp * a.tc_tiles / a.tc_splits), j1 = (int)((long long)(sp + 1) * a.tc_tiles / a.tc_splits);
-  const int n = j1 - j0;  // >= 1: there are no more splits than tiles
-  const int R = a.rows * a.g, r0 = pair * 2 * kTcRows;
-  const int active = R - r0 > kTcRows ? 2 : 1;
-
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::SLOTS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(&q_full, active * kTcRows);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], kHalf);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kTcRows);
+      mbar_init(&p_full[i], kHalf);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(&drained, 1);
-    s_fail = s_issued = 0;
+    s_fail = s_issued = s_odd = 0;
     fence_mbar_init();
     tma_prefetch_map(&tk);
     tma_prefetch_map(&tv);
@@ -139,215 +209,349 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   griddep_wait();
   griddep_launch_dependents();  // behind the wait: what runs next may read the inputs at once
-  // pages that do not exist: their keys are masked, which costs lookups, so only where there are any
-  const int p0 = j0 * kTcKeys / a.kv.page_size, p1 = (j1 * kTcKeys - 1) / a.kv.page_size + 1;
-  bool bad = false;
-  for (int p = p0 + (int)threadIdx.x; p < p1; p += kTcThreads) {
-    const int page = __ldg(a.prefix_pages + p);
-    bad |= page < 0 || page >= a.kv.n_pages;
+  BatchTable table;
+  table.cum = reinterpret_cast<int*>(smem + (2 + C::SLOTS) * C::TILE);
+  table.q0 = table.cum + a.b.batch + 1;
+  table.len = table.q0 + a.b.batch + 1;
+  int own_units = 0;
+  if (a.tc.own_lo < a.tc.own_hi) {
+    const bool bad = batch_table<kTcThreads>(a, table);
+    own_units = line_table<kTcThreads, kTcRows, kTcKeys>(a, a.tc, table, bad, s_scan);
   }
-  bad = __syncthreads_or(bad);
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   volatile int* fail = &s_fail;
+  const Line<kTcRows, kTcKeys> line{a, a.tc, table};
+  auto share = [&](int units, int first) {
+    const int ctas = min((int)gridDim.x, units), c = blockIdx.x;  // fewer units than CTAs: one each, no run is empty
+    return c < ctas ? make_int2(first + cta_first(c, units, ctas), first + cta_first(c + 1, units, ctas)) : make_int2(0, 0);
+  };
+  const int2 run_own = share(own_units, a.tc.prefix_units), run_prefix = share(a.tc.prefix_units, 0);
 
-  if (warp == 8) {
-    // producer: tile n of the ring is K (even) or V (odd) of key tile j0 + n / 2
-    const int box = min(a.kv.page_size, kTcKeys), boxes = kTcKeys / box;
-    auto page_of = [&](int j) {
-      int page = 0;
-      if (lane < boxes && j < j1) {
-        page = __ldg(a.prefix_pages + (j * kTcKeys + lane * box) / a.kv.page_size);
-        if (page < 0 || page >= a.kv.n_pages) page = a.kv.n_pages;  // out of the map: zeros
-      }
-      return page;
-    };
-    int page = page_of(j0);
-    for (int x = 0; x < 2 * n; ++x) {
-      const int s = x % C::SLOTS, r = x / C::SLOTS, j = j0 + (x >> 1);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == 8) {
+      // producer: entry x of the ring is K (even) or V (odd) of the run's key tile x / 2
+      const int box = min(a.kv.page_size, kTcKeys), boxes = kTcKeys / box;
+      int x = 0;
       bool ok = true;
+      for (Segs g(line, run_own, run_prefix); ok && g.valid(); g.next()) {
+        const Seg& s = g.s;
+        const int32_t* pages = page_row(a, s.c);
+        auto page_of = [&](int j) {
+          int page = a.kv.n_pages;  // out of the map: zeros
+          const int key = j * kTcKeys + lane * box;
+          if (lane < boxes && key < s.c.limit) {
+            page = __ldg(pages + key / a.kv.page_size);
+            if (page < 0 || page >= a.kv.n_pages) page = a.kv.n_pages;
+          }
+          return page;
+        };
+        int page = s.n() ? page_of(s.t0) : 0;
+        for (int j = s.t0; ok && j < s.e1; ++j) {
+          int next = 0;
+          for (int v = 0; ok && v < 2; ++v, ++x) {
+            const int slot = x % C::SLOTS, r = x / C::SLOTS;
+            if (lane == 0) {
+              ok = r == 0 || mbar_wait_bounded(&empty[slot], (r - 1) & 1, kWaitLimitNs);
+              if (ok) {
+                mbar_arrive_expect_tx(&full[slot], C::TILE);
+                s_issued = x + 1;
+              } else {
+                *fail = 1;
+              }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
+            if (v == 0 && j + 1 < s.e1) next = page_of(j + 1);
+            if (lane < boxes) {
+              const int at = (j * kTcKeys + lane * box) % a.kv.page_size;
+              const uint32_t dst = base + (2 + slot) * C::TILE + lane * box * 128;
+  #pragma unroll
+              for (int c = 0; c < C::HALVES; ++c) tma_load_4d(dst + c * C::ATOM, v ? &tv : &tk, 64 * c, at, s.c.h, page, &full[slot]);
+            }
+          }
+          page = next;
+        }
+      }
+      __syncwarp();
+    } else if (warp == 9) {
       if (lane == 0) {
-        ok = r == 0 || mbar_wait_bounded(&empty[s], (r - 1) & 1, kWaitLimitNs);
-        if (ok) mbar_arrive_expect_tx(&full[s], C::TILE);
+        constexpr uint32_t bf = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+        constexpr uint32_t idesc_s = idesc_f16_f32(kHalf, kTcKeys, false, false) | bf;
+        constexpr uint32_t idesc_o = idesc_f16_f32(kHalf, HD, false, true) | bf;
+        auto slot = [&](int x) { return base + (2 + x % C::SLOTS) * C::TILE; };
+        auto wait_full = [&](int x) { return mbar_wait_bounded(&full[x % C::SLOTS], (x / C::SLOTS) & 1, kWaitLimitNs); };
+        auto qk = [&](int i, int x) {
+          const uint32_t q = base + i * C::TILE, k = slot(x);
+  #pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (kk / 4) * C::ATOM + (kk % 4) * 32;
+            tc_mma_f16(tmem + kS + 128 * i, sw128_desc(q + off, 16, 1024), sw128_desc(k + off, 16, 1024), idesc_s, kk != 0);
+          }
+          tc_commit(&s_full[i]);
+        };
+        auto pv = [&](int i, int x, bool first) {
+          const uint32_t v = slot(x);
+  #pragma unroll
+          for (int kk = 0; kk < kTcKeys / 16; ++kk)
+            tc_mma_f16_ta(tmem + kO + HD * i, tmem + kS + 128 * i + 8 * kk, sw128_desc(v + kk * 2048, C::ATOM, 1024),
+                          idesc_o, !(first && kk == 0));
+        };
+        int x = 0, items = 0, items1 = 0, tiles = 0, tiles1 = 0;  // so far; ...1: those with a second half
+        bool ok = true;
+        for (Segs g(line, run_own, run_prefix); ok && g.valid(); g.next()) {
+          const int n = g.s.n(), active = g.s.active();
+          if (n == 0) continue;
+          ok = wait_full(x);
+          for (int i = 0; ok && i < active; ++i) {
+            ok = mbar_wait_bounded(&q_full[i], (i ? items1 : items) & 1, kWaitLimitNs);
+            if (!ok) break;
+            tc_fence_after();
+            qk(i, x);
+          }
+          if (ok) tc_commit(&empty[x % C::SLOTS]);
+          for (int j = 0; ok && j < n; ++j) {
+            const int xv = x + 2 * j + 1, xk = xv + 1;
+            ok = wait_full(xv);
+            for (int i = 0; ok && i < active; ++i) {
+              ok = mbar_wait_bounded(&p_full[i], ((i ? tiles1 : tiles) + j) & 1, kWaitLimitNs);
+              if (ok && i == 0 && j + 1 < n) ok = wait_full(xk);
+              if (!ok) break;
+              tc_fence_after();
+              pv(i, xv, j == 0);
+              if (j + 1 < n)
+                qk(i, xk);
+              else
+                tc_commit(&o_full[i]);
+            }
+            if (ok) {
+              tc_commit(&empty[xv % C::SLOTS]);
+              if (j + 1 < n) tc_commit(&empty[xk % C::SLOTS]);
+            }
+          }
+          x += 2 * n;
+          tiles += n, ++items;
+          if (active == 2) tiles1 += n, ++items1;
+        }
+        if (!ok) {  // let what was issued end before the TMEM goes back
+          *fail = 1;
+          tc_commit(&drained);
+          mbar_wait_bounded(&drained, 0, kWaitLimitNs);
+        }
       }
-      if (!__shfl_sync(0xffffffffu, ok, 0)) {
-        if (lane == 0) *fail = 1;
-        break;
-      }
-      const int next = x & 1 ? page_of(j + 1) : page;
-      if (lane < boxes) {
-        const int slot = (j * kTcKeys + lane * box) % a.kv.page_size;
-        const uint32_t dst = base + (2 + s) * C::TILE + lane * box * 128;
-#pragma unroll
-        for (int c = 0; c < C::HALVES; ++c)
-          tma_load_4d(dst + c * C::ATOM, x & 1 ? &tv : &tk, 64 * c, slot, h, page, &full[s]);
-      }
-      page = next;
-      if (lane == 0) s_issued = x + 1;
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp == 9) {
-    if (lane == 0) {
-      constexpr uint32_t bf = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
-      constexpr uint32_t idesc_s = idesc_f16_f32(kTcRows, kTcKeys, false, false) | bf;
-      constexpr uint32_t idesc_o = idesc_f16_f32(kTcRows, HD, false, true) | bf;
-      auto slot = [&](int x) { return base + (2 + x % C::SLOTS) * C::TILE; };
-      auto wait_full = [&](int x) { return mbar_wait_bounded(&full[x % C::SLOTS], (x / C::SLOTS) & 1, kWaitLimitNs); };
-      auto qk = [&](int i, int x) {
-        const uint32_t q = base + i * C::TILE, k = slot(x);
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk / 4) * C::ATOM + (kk % 4) * 32;
-          tc_mma_f16(tmem + kS + 128 * i, sw128_desc(q + off, 16, 1024), sw128_desc(k + off, 16, 1024), idesc_s, kk != 0);
-        }
-        tc_commit(&s_full[i]);
-      };
-      auto pv = [&](int i, int x, bool first) {
-        const uint32_t v = slot(x);
-#pragma unroll
-        for (int kk = 0; kk < kTcKeys / 16; ++kk)
-          tc_mma_f16_ta(tmem + kO + HD * i, tmem + kS + 128 * i + 8 * kk, sw128_desc(v + kk * 2048, C::ATOM, 1024),
-                        idesc_o, !(first && kk == 0));
-      };
-      bool ok = mbar_wait_bounded(&q_full, 0, kWaitLimitNs) && wait_full(0);
-      if (ok) {
-        tc_fence_after();
-        for (int i = 0; i < active; ++i) qk(i, 0);
-        tc_commit(&empty[0]);
-      }
-      for (int j = 0; ok && j < n; ++j) {
-        const int xv = 2 * j + 1, xk = 2 * j + 2;
-        ok = wait_full(xv);
-        for (int i = 0; ok && i < active; ++i) {
-          ok = mbar_wait_bounded(&p_full[i], j & 1, kWaitLimitNs);
-          if (ok && i == 0 && j + 1 < n) ok = wait_full(xk);
-          if (!ok) break;
-          tc_fence_after();
-          pv(i, xv, j == 0);
-          if (j + 1 < n)
-            qk(i, xk);
-          else
-            tc_commit(&o_full[i]);
-        }
-        if (ok) {
-          tc_commit(&empty[xv % C::SLOTS]);
-          if (j + 1 < n) tc_commit(&empty[xk % C::SLOTS]);
-        }
-      }
-      if (!ok) {  // let what was issued end before the TMEM goes back
-        *fail = 1;
-        tc_commit(&drained);
-        mbar_wait_bounded(&drained, 0, kWaitLimitNs);
-      }
-    }
-    __syncwarp();
-  } else if (warp / 4 < active) {
-    const int i = warp / 4, row = (warp & 3) * 32 + lane, r = r0 + i * kTcRows + row;
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int i = warp / 4, row = (warp & 3) * 32 + lane;
     const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kS + 128 * i;
     const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kO + HD * i;
-    const int t = r / a.g, head = h * a.g + r - t * a.g;
-    {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (long long)t * a.q_stride +
-                                                        (long long)head * a.q_head_stride);
-      uint8_t* dst = smem + i * C::TILE + row * 128;
+    auto load_q = [&](const Seg& s) {
+      if (i >= s.active() || s.n() == 0) return;
+      // Lane l finds row l of its warp; then HD / 8 lanes take a row, so that a load covers whole rows, all loads in flight
+      // at once (they queue behind the first K and V tiles of all CTAs).
+      constexpr int LANES = HD / 8, ROWS = 32 / LANES;
+      const int rr = s.c.rt * kTcRows + i * kHalf + row, j = rr / a.g, c = lane % LANES;
+      const long long mine = i * kHalf + row < s.c.nrows
+                                 ? (s.c.q0 + j) * a.q_stride + (s.c.h * a.g + rr - j * a.g) * a.q_head_stride
+                                 : -1;
+      uint4 v[32 / ROWS];
 #pragma unroll
-      for (int c = 0; c < HD / 8; ++c) {
-        const uint4 v = r < R ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + (c / 8) * C::ATOM + (((c % 8) ^ (row & 7)) << 4)) = v;
+      for (int y = 0; y < 32 / ROWS; ++y) {
+        const long long off = __shfl_sync(0xffffffffu, mine, y * ROWS + lane / LANES);
+        v[y] = off >= 0 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + off) + c) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int y = 0; y < 32 / ROWS; ++y) {
+        const int rw = (warp & 3) * 32 + y * ROWS + lane / LANES;
+        *reinterpret_cast<uint4*>(smem + i * C::TILE + rw * 128 + (c / 8) * C::ATOM + (((c % 8) ^ (rw & 7)) << 4)) = v[y];
       }
       fence_async_smem();
-      mbar_arrive(&q_full);
-    }
-    float m = -INFINITY, l = 0.0f;
+      mbar_arrive(&q_full[i]);
+    };
+    int x = 0, tiles = 0, items = 0;  // ring entries so far; tiles and items of this half
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      ok = mbar_wait_bounded(&s_full[i], j & 1, kWaitLimitNs);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
+    Segs g(line, run_own, run_prefix);
+    if (g.valid()) load_q(g.s);
+    while (g.valid()) {
+      const Seg s = g.s;
+      const int n = s.n();
+      g.next();
+      if (i >= s.active()) {
+        x += 2 * n;
+        if (g.valid()) load_q(g.s);
+        continue;
       }
-      tc_fence_after();
-      uint32_t s[4][32];
+      const int lim = row_limit(a, s.c, i * kHalf + row, kTcRows);
+      const int32_t* pages = page_row(a, s.c);
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; ok && j < n; ++j) {
+        const int key0 = (s.t0 + j) * kTcKeys;
+        // a lane looks at the page of four keys (pages hold a multiple of 8)
+        int page = 0;
+        if (key0 + 4 * lane < s.c.limit) page = __ldg(pages + (key0 + 4 * lane) / a.kv.page_size);
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0 && page < a.kv.n_pages);
+        const bool edge = key0 + kTcKeys > s.c.first;  // some row does not see all of the tile's keys
+        if (edge) {
+          const int xv = x + 2 * j + 1;
+          ok = mbar_wait_bounded(&full[xv % C::SLOTS], (xv / C::SLOTS) & 1, kWaitLimitNs);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          // V of the keys that not every row sees: zeros behind the last one, and over what is not finite
+          constexpr int ROW = 8 * C::HALVES;  // 16-byte chunks of a row
+          const int from = max(s.c.first - key0, 0), to = min(s.c.limit - key0, kTcKeys);
+          uint8_t* v = smem + (2 + xv % C::SLOTS) * C::TILE;
+          auto chunk = [&](int y) { return reinterpret_cast<uint4*>(v + (y % ROW / 8) * C::ATOM + y / ROW * 128 + (y % 8) * 16); };
+          uint32_t odd = 0;
+#pragma unroll 4
+          for (int y = from * ROW + row; y < to * ROW; y += kHalf) {
+            const uint4 w = *chunk(y);
+            odd |= odd_bits<T>(w.x) | odd_bits<T>(w.y) | odd_bits<T>(w.z) | odd_bits<T>(w.w);
+          }
+          for (int y = to * ROW + row; y < kTcKeys * ROW; y += kHalf) *chunk(y) = make_uint4(0, 0, 0, 0);
+          if (odd & 0x80008000u) {
+            *reinterpret_cast<volatile int*>(&s_odd) = 1;
+            for (int y = from * ROW + row; y < to * ROW; y += kHalf) {
+              const uint4 old = *chunk(y);
+              uint32_t w[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_async(ts + 32 * c, s[c]);
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t bits = odd_bits<T>(w[e]);
+                if (bits & 0x8000u) w[e] &= 0xFFFF0000u;
+                if (bits & 0x80000000u) w[e] &= 0x0000FFFFu;
+              }
+              *chunk(y) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          fence_async_smem();
+        }
+        ok = mbar_wait_bounded(&s_full[i], (tiles + j) & 1, kWaitLimitNs);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sc[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_wait(s[c]);
-      if (bad) {
+        for (int c = 0; c < 4; ++c) tmem_ld_async(ts + 32 * c, sc[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait(sc[c]);
+        if (edge) {
+          const int vis = lim - key0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * c + e >= vis) sc[c][e] = 0xff800000u;
+        }
+        if (there != 0xffffffffu) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((there >> (8 * c + e / 4)) & 1)) sc[c][e] = 0xff800000u;
+        }
+        float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int page = __ldg(a.prefix_pages + ((j0 + j) * kTcKeys + 32 * c + lane) / a.kv.page_size);
-          const unsigned there = __ballot_sync(0xffffffffu, page >= 0 && page < a.kv.n_pages);
+          mx[c] = __uint_as_float(sc[c][0]);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((there >> e) & 1)) s[c][e] = 0xff800000u;
+          for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(sc[c][e]));
         }
-      }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][e]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
-      if (__any_sync(0xffffffffu, top > m + kSlack || (m == -INFINITY && top > m))) {
-        const float nm = fmaxf(m, top), f = m == -INFINITY ? 0.0f : ex2(m - nm);
-        m = nm;
-        l *= f;
-        if (j > 0) {  // PV of the tile before has ended: its S followed it
+        const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float top = best * a.scale2;
+        if (__any_sync(0xffffffffu, top > m + kSlack || (m == -INFINITY && top > m))) {
+          const float nm = fmaxf(m, top), f = m == -INFINITY ? 0.0f : ex2(m - nm);
+          m = nm;
+          l *= f;
+          if (j > 0) {  // PV of the tile before has ended: its S followed it
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_async(to + 32 * c, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st_32(to + 32 * c, o);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // P's 16 columns lie over columns of S that have been read
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float y0 = ex2(fmaf(__uint_as_float(sc[c][2 * e]), a.scale2, -ref));
+            const float y1 = ex2(fmaf(__uint_as_float(sc[c][2 * e + 1]), a.scale2, -ref));
+            sum[e & 3] += y0 + y1;
+            p[e] = Half16<T>::pack(y0, y1);
+          }
+          tmem_st_16(ts + 16 * c, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[i]);
+      }
+      if (ok && g.valid()) load_q(g.s);  // the item's products with Q have ended
+      if (ok && n > 0) {
+        ok = mbar_wait_bounded(&o_full[i], items & 1, kWaitLimitNs);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      if (!ok) {
+        *fail = 1;
+        l = __int_as_float(0x7fffffff);  // a row whose work gave up is NaN, not stale
+      }
+      const Dest d = dest<kTcRows>(a, s.c, s.t0 == 0, s.t1 == s.c.tiles, s.c.b < 0 ? 0 : gridDim.x, a.tc_o, a.tc_ml, HD);
+      const bool on = i * kHalf + row < s.c.nrows;
+      const long long at = on ? d.row(i * kHalf + row) : 0;
+      const bool odd = *reinterpret_cast<volatile int*>(&s_odd) != 0;
+      if (ok) {
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          if (n > 0) {
             tmem_ld_async(to + 32 * c, o);
             tmem_ld_wait(o);
+          } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st_32(to + 32 * c, o);
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          if (odd) {  // what the zeros written over V took from the rows that see it
+            for (int key = max(s.c.first, s.t0 * kTcKeys); key < min(lim, s.e1 * kTcKeys); ++key) {
+              const int page = __ldg(pages + key / a.kv.page_size);
+              if (page < 0 || page >= a.kv.n_pages) continue;
+              const uint32_t* v = reinterpret_cast<const uint32_t*>(
+                  static_cast<const T*>(a.kv.v) + page * a.kv.page_stride + (key % a.kv.page_size) * a.kv.slot_stride +
+                  s.c.h * a.kv.head_stride + 32 * c);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const uint32_t w = __ldg(v + e);
+                const float2 f = Half16<T>::unpack(w);
+                if (odd_bits<T>(w) & 0x8000u) o[2 * e] = __float_as_uint(__uint_as_float(o[2 * e]) + f.x);
+                if (odd_bits<T>(w) & 0x80000000u) o[2 * e + 1] = __float_as_uint(__uint_as_float(o[2 * e + 1]) + f.y);
+              }
+            }
+          }
+          if (on) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st_8(d.o + at * HD + 32 * c + 8 * e, o + 8 * e);
           }
         }
       }
-      const float ref = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        uint32_t p[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float x = ex2(fmaf(__uint_as_float(s[c + e / 16][2 * e % 32]), a.scale2, -ref));
-          const float y = ex2(fmaf(__uint_as_float(s[c + e / 16][2 * e % 32 + 1]), a.scale2, -ref));
-          sum[e & 3] += x + y;
-          p[e] = Half16<T>::pack(x, y);
-        }
-        tmem_st_32(ts + 16 * c, p);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&p_full[i]);
+      if (on) d.ml[at] = make_float2(m, l);
+      tc_fence_before();  // O has been read: the next item's first PV waits for this half's P
+      x += 2 * n;
+      tiles += n;
+      if (n > 0) ++items;
     }
-    if (ok) ok = mbar_wait_bounded(&o_full[i], 0, kWaitLimitNs);
-    ok = __all_sync(0xffffffffu, ok);
-    const long long at = (long long)sp * a.rows * a.H + (long long)t * a.H + head;
-    if (ok) {
-      tc_fence_after();
-#pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld_async(to + 32 * c, o);
-        tmem_ld_wait(o);
-        if (r < R) {
-          float4* dst = reinterpret_cast<float4*>(a.tc_o + at * HD + 32 * c);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                                 __uint_as_float(o[4 * e + 3]));
-        }
-      }
-    } else {
-      *fail = 1;
-      l = __int_as_float(0x7fffffff);  // a row whose work gave up is NaN, not stale
-    }
-    if (r < R) a.tc_ml[at] = make_float2(m, l);
   }
   tc_fence_before();
   __syncthreads();
@@ -370,9 +574,15 @@ int launch(const PrefixArgs& a, cudaStream_t st) {
   if (int rc = make_tmap_pages(&tv, a.kv, a.kv.v, box)) return rc;
   auto kern = prefix_tc_kernel<T, HD>;
   static std::atomic<unsigned long long> done;
-  cudaError_t e = set_max_dynamic_smem(kern, TcCfg<HD>::SMEM, done);
-  if (e == cudaSuccess)
-    e = launch_pdl(kern, dim3(a.Hkv * a.tc_pairs * a.tc_splits), dim3(kTcThreads), TcCfg<HD>::SMEM, st, tk, tv, a);
+  // the register split needs the launch registers that it was laid out for
+  static const int regs = [&] {
+    cudaFuncAttributes f = {};
+    return cudaFuncGetAttributes(&f, kern) == cudaSuccess ? f.numRegs : 0;
+  }();
+  if (regs != kRegsLaunch) return set_error(Q4B_EUNSUPPORTED, "prefix_attention: built with %d registers, not %d", regs, kRegsLaunch);
+  const int table = a.tc.own_lo < a.tc.own_hi ? 12 * (a.b.batch + 1) : 0;
+  cudaError_t e = set_max_dynamic_smem(kern, TcCfg<HD>::SMEM + 12 * (kTcMaxBatch + 1), done);
+  if (e == cudaSuccess) e = launch_pdl(kern, dim3(a.tc_ctas), dim3(kTcThreads), TcCfg<HD>::SMEM + table, st, tk, tv, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(Q4B_ELAUNCH, "prefix_attention: launch failed: %s", cudaGetErrorString(e));
@@ -382,25 +592,13 @@ int launch(const PrefixArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-PrefixTcPlan prefix_tc_plan(int rows, int H, int prefix_len, const q4b_paged_kv& kv) {
-  PrefixTcPlan p = {0, 0, 0};
-  const int R = rows * (H / kv.n_kv_heads), ps = kv.page_size;
-  const int tiles = prefix_len / kTcKeys;
-  // Pages that a 128-key tile holds whole, or that hold whole tiles, in boxes of full swizzle groups (8 rows);
-  // strides that a tensor map can describe.
+// Pages that a 128-key tile holds whole, or that hold whole tiles, in boxes of full swizzle groups (8 rows);
+// strides that a tensor map can describe.
+bool prefix_tc_takes(const q4b_paged_kv& kv) {
+  const int ps = kv.page_size;
   const bool boxes = ps % 8 == 0 && (ps % kTcKeys == 0 || kTcKeys % ps == 0);
   const bool strides = kv.slot_stride > 0 && (kv.n_kv_heads == 1 || kv.head_stride > 0) && (kv.n_pages == 1 || kv.page_stride > 0);
-  if (kv.head_dim < 64 || !boxes || !strides || tiles == 0 || R < kTcMinRows) return p;
-  p.tiles = tiles;
-  p.pairs = (R + 2 * kTcRows - 1) / (2 * kTcRows);
-  // Splits: the fewest rounds of (tiles + 3 tiles' worth of start and end) over the SMs.
-  const int items = kv.n_kv_heads * p.pairs;
-  double best = 0;
-  for (int s = 1; s <= tiles && s <= kTcMaxSplits; ++s) {
-    const double cost = (double)((items * (long long)s + 147) / 148) * ((tiles + s - 1) / s + 3);
-    if (s == 1 || cost < best) best = cost, p.splits = s;
-  }
-  return p;
+  return kv.head_dim >= 64 && boxes && strides;
 }
 
 int prefix_tc_run(const PrefixArgs& a, cudaStream_t st) {

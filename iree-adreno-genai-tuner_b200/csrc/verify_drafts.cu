@@ -5,15 +5,16 @@
 //   w = max(p - d, 0) of that row (p of the last row if all were kept): the first j with W_j > u W_{V-1}, W the
 //   running sum of w.
 //
-// The sums have 43 bits and more (64-bit words where it matters, pairs of fp32 words over the values of a
+// The sums have 40 bits and more (64-bit words where it matters, pairs of fp32 words over the values of a
 // lane): a running sum of 10^5 probabilities in fp32 is off by more than a typical w, and the
 // drawn index would depend on the order of the sum. The products u d of the tests are exact in 64 bits.
 //
 // Bound by memory: one row of p, and of d where a draft was rejected, per sequence; the acceptance tests read
 // two numbers per draft. A cluster of CTAs takes one sequence, so that a row's read is spread over several
-// SMs in one launch: each CTA sums its slice in tiles of 1024 values (a warp per tile, the tile sums stay
-// in shared memory), the slices' sums meet through distributed shared memory, and the CTA whose slice holds
-// the drawn index reads that one tile again (from L2) to find it.
+// SMs in one launch: each warp sums an equal piece of the row, the pieces' sums go to every CTA through
+// distributed shared memory, and the CTA whose warp holds the drawn index reads that piece again (from L2),
+// a few values a thread, to find it. What is left is latency: offsets, tokens, the tested numbers, the row, the
+// exchange and the piece are dependent reads (8 us for one sequence).
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -22,9 +23,8 @@ namespace q4b {
 namespace {
 
 constexpr int kVfThreads = 256, kVfWarps = kVfThreads / 32;
-constexpr int kTile = 1024;                  // values per tile
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 8, kMaxPieces = kMaxCluster * kVfWarps;
 
 struct VerifyArgs {
   const void *target, *draft;
@@ -74,17 +74,18 @@ __device__ __forceinline__ void unpack16(const uint4& v, float (&x)[N]) {
   }
 }
 
-// A sum in two fp32 words. The error of each fp32 addition and subtraction is itself an fp32 number, found
-// by Knuth's two-sum; the errors are added up in `lo`. Over the 32 values of a lane hi + lo is off by
-// less than 2^-43 of the sum, far below the share of one token, at fp32 speed: conversions to 64
-// bits and 64-bit additions for every value took three times as long as the row's read.
+// A sum in two fp32 words. The error of an fp32 addition or subtraction is itself an fp32 number, found by
+// Dekker's fast two-sum (of numbers a >= b >= 0, s = a + b: b - (s - a), and s = a - b: (a - s) - b); the errors
+// are added up in `lo`. Over a lane's few hundred values hi + lo is off by less than 2^-40 of the sum, far
+// below the share of one token, at fp32 speed: conversions to 64 bits and 64-bit additions for every value
+// took three times as long as the row's read.
 struct Sum2 {
   float hi = 0.0f, lo = 0.0f;
-  float top = 0.0f;  // largest value met: an infinite one sends the tile to the careful sum
-  __device__ __forceinline__ void add(float x, float e) {
-    const float s = __fadd_rn(hi, x), b = __fsub_rn(s, hi);
-    lo = __fadd_rn(lo, __fadd_rn(__fadd_rn(__fsub_rn(hi, __fsub_rn(s, b)), __fsub_rn(x, b)), e));
-    hi = s;
+  float top = 0.0f;  // largest value met: an infinite one sends the piece to the careful sum
+  __device__ __forceinline__ void add(float x, float e) {  // x >= 0
+    const float a = fmaxf(hi, x), b = fminf(hi, x);
+    hi = __fadd_rn(a, b);
+    lo = __fadd_rn(lo, __fadd_rn(__fsub_rn(b, __fsub_rn(hi, a)), e));
   }
   __device__ __forceinline__ void add_target(float p) {
     p = fmaxf(p, 0.0f);  // NaN and negative: zero
@@ -94,58 +95,70 @@ struct Sum2 {
   __device__ __forceinline__ void add_rest(float p, float d) {
     p = fmaxf(p, 0.0f), d = fmaxf(d, 0.0f);
     top = fmaxf(top, fmaxf(p, d));
-    const float s = __fsub_rn(p, d), b = __fsub_rn(s, p);
-    const float e = __fsub_rn(__fsub_rn(p, __fsub_rn(s, b)), __fadd_rn(d, b));
-    if (s > 0.0f) add(s, e);  // the rounded difference has the exact one's sign
+    const float s = __fsub_rn(p, d);  // has the exact difference's sign
+    if (s > 0.0f) add(s, __fsub_rn(__fsub_rn(p, s), d));
   }
 };
 
-// This lane's share of the weights of tile [lo, lo + kTile), whose bounds are 16-byte aligned in p and d: every
-// 32nd vector (coalesced), or, with `runs`, the 32 values from lo + 32 lane.
+// A row cut into equal pieces, at 16-byte vectors where p and d are aligned alike (the first piece then takes the values
+// in front of the first vector too, the last one those behind the last), else at single values (vectors 0).
 template <typename T>
-__device__ __forceinline__ double lane_sum_vec(const Weights<T>& w, int lo, int lane, bool runs) {
-  constexpr int N = 16 / sizeof(T), U = kTile / (32 * N), HALF = U / 2;
+struct Row {
+  static constexpr int N = 16 / sizeof(T);
+  int vocab, pieces, head, vectors;
+  __device__ __forceinline__ Row(const Weights<T>& w, int vocab, int pieces) : vocab(vocab), pieces(pieces) {
+    const int mis = (int)(reinterpret_cast<uintptr_t>(w.p) % 16 / sizeof(T));
+    head = min(mis ? N - mis : 0, vocab);
+    vectors = (vocab - head) / N;
+    if (w.d && reinterpret_cast<uintptr_t>(w.d) % 16 != reinterpret_cast<uintptr_t>(w.p) % 16) vectors = 0;
+  }
+  __device__ __forceinline__ int vector(int k) const { return (int)((long long)vectors * k / pieces); }
+  __device__ __forceinline__ int value(int k) const {
+    if (k == 0) return 0;
+    if (k == pieces) return vocab;
+    return vectors ? head + vector(k) * N : (int)((long long)vocab * k / pieces);
+  }
+};
+
+// A lane's share of the weights of vectors [lo, hi), every 32nd; four 16-byte loads in flight.
+template <typename T, bool REST>
+__device__ __forceinline__ double lane_sum(const Weights<T>& w, int head, int lo, int hi, int lane) {
+  constexpr int N = 16 / sizeof(T), U = REST ? 2 : 4;
+  const T* p = w.p + head;
+  const T* d = REST ? w.d + head : nullptr;
   Sum2 sum;
+  for (int v0 = lo + lane; v0 < hi; v0 += 32 * U) {
+    uint4 pv[U], dv[U];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint4 pv[HALF], dv[HALF];
-    auto first = [&](int u) { return lo + N * (runs ? lane * U + h * HALF + u : (h * HALF + u) * 32 + lane); };
-#pragma unroll
-    for (int u = 0; u < HALF; ++u) {
-      pv[u] = ld_stream_u4(w.p + first(u));
-      if (w.d) dv[u] = ld_stream_u4(w.d + first(u));
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + 32 * u;
+      pv[u] = dv[u] = make_uint4(0, 0, 0, 0);
+      if (v < hi) pv[u] = ld_stream_u4(p + (long long)v * N);
+      if (REST && v < hi) dv[u] = ld_stream_u4(d + (long long)v * N);
     }
 #pragma unroll
-    for (int u = 0; u < HALF; ++u) {
+    for (int u = 0; u < U; ++u) {
       float a[N];
       unpack16<T>(pv[u], a);
-      if (w.d) {
+      if constexpr (REST) {
         float b[N];
         unpack16<T>(dv[u], b);
 #pragma unroll
         for (int i = 0; i < N; ++i) sum.add_rest(a[i], b[i]);
       } else {
-        const unsigned at = (unsigned)(w.skip - first(u));
+        const unsigned at = (unsigned)(w.skip - head - (v0 + 32 * u) * N);
 #pragma unroll
         for (int i = 0; i < N; ++i) sum.add_target(at == (unsigned)i ? 0.0f : a[i]);
       }
     }
   }
-  const bool odd = !(sum.top < INFINITY && sum.hi < INFINITY);
-  if (__any_sync(0xffffffffu, odd)) {  // an infinite value counts as zero
+  if (!(sum.top < INFINITY && sum.hi < INFINITY)) {  // an infinite value counts as zero
     double s = 0.0;
-    for (int i = 0; i < kTile / 32; ++i) s += w.at(lo + (runs ? lane * (kTile / 32) + i : i * 32 + lane));
+    for (int v = lo + lane; v < hi; v += 32)
+      for (int i = 0; i < N; ++i) s += w.at(head + v * N + i);
     return s;
   }
   return (double)sum.hi + (double)sum.lo;
-}
-
-template <typename T>
-__device__ __forceinline__ double tile_sum_any(const Weights<T>& w, int lo, int hi, int lane) {
-  double s = 0.0;
-#pragma unroll 8
-  for (int i = lo + lane; i < hi; i += 32) s += w.at(i);
-  return s;
 }
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -165,16 +178,15 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads, 4) verify_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kVfThreads, 5) verify_kernel(VerifyArgs a) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / nc;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __shared__ double s_tile[kMaxVocab / kTile + 2];  // this CTA's tile sums
-  __shared__ double s_cta[2][kMaxCluster];          // every CTA's sum (twice: the residual, then the target)
+  __shared__ double s_piece[2][kMaxPieces];  // every warp's sum (twice: the residual, then the target)
   __shared__ double s_part[kVfWarps];
-  __shared__ int s_kept;
+  __shared__ int s_kept, s_first, s_some;
   cluster.barrier_arrive();  // waited for before the first write to another CTA: by then all have started
   griddep_launch_dependents();
   griddep_wait();
@@ -206,7 +218,11 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_kernel(VerifyArgs a) {
         break;
       }
     }
-    if (lane == 0) s_kept = kept;
+    if (lane == 0) {
+      s_kept = kept;
+      s_first = kVfThreads;
+      s_some = 0;
+    }
   }
   __syncthreads();
   const int kept = s_kept;
@@ -217,42 +233,34 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_kernel(VerifyArgs a) {
   w.d = cut && a.draft ? static_cast<const T*>(a.draft) + row * a.draft_stride : nullptr;
   w.skip = cut && !a.draft ? __ldg(a.tokens + row + 1) : -1;
 
-  // Tiles: `head` values up to p's first 16-byte boundary, then tiles of 1024, the last one short. Where d
-  // is aligned otherwise than p, no tile takes the vector path.
-  constexpr int N = 16 / sizeof(T);
-  const int mis = (int)((reinterpret_cast<uintptr_t>(w.p) % 16) / sizeof(T));
-  const int head = min(mis ? N - mis : 0, a.vocab);
-  const int tiles = 1 + (a.vocab - head + kTile - 1) / kTile;
-  const int t_lo = (int)((long long)tiles * rank / nc), t_hi = (int)((long long)tiles * (rank + 1) / nc);
-  auto lo_of = [&](int t) { return t == 0 ? 0 : head + (t - 1) * kTile; };
-  auto hi_of = [&](int t) { return t == 0 ? head : min(head + t * kTile, a.vocab); };
-
-  double base = 0.0, total = 0.0;
+  const int pieces = nc * kVfWarps, piece = rank * kVfWarps + warp;
+  double total = 0.0, before = 0.0;  // before: of the pieces in front of this lane's two
+  double mine0 = 0.0, mine1 = 0.0;   // pieces 2 lane and 2 lane + 1
   int round = 0;
   for (;; ++round) {
-    const bool vec = !w.d || reinterpret_cast<uintptr_t>(w.d) % 16 == reinterpret_cast<uintptr_t>(w.p) % 16;
-    double mine = 0.0;
-    for (int t = t_lo + warp; t < t_hi; t += kVfWarps) {
-      const int lo = lo_of(t), hi = hi_of(t);
-      const double s = warp_sum(vec && hi - lo == kTile ? lane_sum_vec(w, lo, lane, false) : tile_sum_any(w, lo, hi, lane));
-      if (lane == 0) s_tile[t - t_lo] = s;
-      mine += s;
+    const Row<T> row_of(w, a.vocab, pieces);
+    double s = 0.0;
+    int lo = row_of.value(piece), hi = row_of.value(piece + 1);
+    if (row_of.vectors) {
+      const int v0 = row_of.vector(piece), v1 = row_of.vector(piece + 1), h = row_of.head;
+      s = w.d ? lane_sum<T, true>(w, h, v0, v1, lane) : lane_sum<T, false>(w, h, v0, v1, lane);
+      // the values outside vectors: at most N - 1 in front and behind
+      if (lo + lane < h + v0 * Row<T>::N) s += w.at(lo + lane);
+      if (h + v1 * Row<T>::N + lane < hi) s += w.at(h + v1 * Row<T>::N + lane);
+    } else {
+#pragma unroll 8
+      for (int i = lo + lane; i < hi; i += 32) s += w.at(i);
     }
-    if (lane == 0) s_part[warp] = mine;
-    __syncthreads();
+    s = warp_sum(s);
     if (round == 0) cluster.barrier_wait();
-    if (threadIdx.x < nc) {
-      double s = 0.0;
-      for (int i = 0; i < kVfWarps; ++i) s += s_part[i];
-      *cluster.map_shared_rank(&s_cta[round][rank], threadIdx.x) = s;
-    }
+    if (lane < nc) *cluster.map_shared_rank(&s_piece[round][piece], lane) = s;
     cluster.sync();
-    base = total = 0.0;
-    for (int c = 0; c < nc; ++c) {
-      if (c == rank) base = total;
-      total += s_cta[round][c];
-    }
-    // an empty residual: draw from the target (the same decision in every CTA: they hold the same sums)
+    mine0 = 2 * lane < pieces ? s_piece[round][2 * lane] : 0.0;
+    mine1 = 2 * lane + 1 < pieces ? s_piece[round][2 * lane + 1] : 0.0;
+    const double end = warp_scan(mine0 + mine1, lane);
+    total = __shfl_sync(0xffffffffu, end, 31);
+    before = end - (mine0 + mine1);
+    // an empty residual: draw from the target (the same decision in every warp: they hold the same sums)
     if (total > 0.0 || (!w.d && w.skip < 0)) break;
     w.d = nullptr;
     w.skip = -1;
@@ -270,63 +278,59 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_kernel(VerifyArgs a) {
   }
   if (!(total > 0.0)) return;
 
-  // The CTA whose slice holds the index: the first whose end lies above the mark; where rounding leaves the
-  // mark at the very end, the last slice with any weight (every CTA decides the same).
+  // The piece that holds the index: the first whose end lies above the mark; where rounding leaves the mark at the
+  // very end, the last one with any weight. Every warp decides the same.
   const double mark = (double)__ldg(a.uniforms + r.y - 1) * total;
-  int owner = -1, some = 0;
-  double run = 0.0;
-  for (int c = 0; c < nc; ++c) {
-    run += s_cta[round][c];
-    if (owner < 0 && run > mark) owner = c;
-    if (s_cta[round][c] > 0.0) some = c;
-  }
-  if (owner < 0) owner = some;
-  if (owner != rank || warp != 0) return;
+  auto choose = [&](bool above, bool any, int& lane_of) {  // first lane above, else the last with weight
+    const unsigned m = __ballot_sync(0xffffffffu, above), o = __ballot_sync(0xffffffffu, any);
+    lane_of = m ? __ffs(m) - 1 : 31 - __clz(o);
+    return m != 0;
+  };
+  int f;
+  const double mid = before + mine0, end = mid + mine1;
+  const bool above0 = mine0 > 0.0 && mid > mark, above1 = mine1 > 0.0 && end > mark;
+  const bool found = choose(above0 || above1, mine0 > 0.0 || mine1 > 0.0, f);
+  const bool second = found ? !above0 : mine1 > 0.0;
+  const int at = __shfl_sync(0xffffffffu, 2 * lane + second, f);
+  const double base = __shfl_sync(0xffffffffu, second ? mid : before, f);
+  if (at / kVfWarps != rank) return;
 
-  // its tile, by the same rule
-  int tile = -1, tile_some = t_lo;
-  double cum = base, tile_base = base;
-  for (int t0 = t_lo; t0 < t_hi && tile < 0; t0 += 32) {
-    const double s = t0 + lane < t_hi ? s_tile[t0 + lane - t_lo] : 0.0;
-    const double end = cum + warp_scan(s, lane);
-    const unsigned above = __ballot_sync(0xffffffffu, s > 0.0 && end > mark), any = __ballot_sync(0xffffffffu, s > 0.0);
-    const int f = above ? __ffs(above) - 1 : any ? 31 - __clz(any) : -1;
-    if (f >= 0) {
-      tile_some = t0 + f;
-      tile_base = __shfl_sync(0xffffffffu, end - s, f);
-      if (above) tile = t0 + f;
-    }
-    cum = __shfl_sync(0xffffffffu, end, 31);
-  }
-  if (tile < 0) tile = tile_some;
-
-  // its run of values: lane l sums run l of the tile
-  const int lo = lo_of(tile), hi = hi_of(tile), per = (hi - lo + 31) / 32;
-  const int from = min(lo + lane * per, hi), to = min(from + per, hi);
-  double s = 0.0;
-  if (hi - lo == kTile && (!w.d || reinterpret_cast<uintptr_t>(w.d) % 16 == reinterpret_cast<uintptr_t>(w.p) % 16)) {
-    s = lane_sum_vec(w, lo, lane, true);
-  } else {
+  // Its values again, a run for each thread of the CTA, and the index by the same rule.
+  const Row<T> row_of(w, a.vocab, pieces);
+  const int lo = row_of.value(at), hi = row_of.value(at + 1), share = (hi - lo + kVfThreads - 1) / kVfThreads;
+  const int from = min(lo + (int)threadIdx.x * share, hi), to = min(from + share, hi);
+  double sum = 0.0;
 #pragma unroll 8
-    for (int i = from; i < to; ++i) s += w.at(i);
+  for (int i = from; i < to; ++i) sum += w.at(i);
+  double run = warp_scan(sum, lane);
+  if (lane == 31) s_part[warp] = run;
+  __syncthreads();
+  run += base;
+  for (int k = 0; k < warp; ++k) run += s_part[k];
+  if (sum > 0.0) {
+    atomicMax(&s_some, (int)threadIdx.x);
+    if (run > mark) atomicMin(&s_first, (int)threadIdx.x);
   }
-  double end = tile_base + warp_scan(s, lane);
-  unsigned above = __ballot_sync(0xffffffffu, s > 0.0 && end > mark), any = __ballot_sync(0xffffffffu, s > 0.0);
-  const int f = above ? __ffs(above) - 1 : 31 - __clz(any);
-  // its value: lane l takes value l of the run
-  const int i = __shfl_sync(0xffffffffu, from, f) + lane;
-  const double run_base = __shfl_sync(0xffffffffu, end - s, f);
-  s = i < __shfl_sync(0xffffffffu, to, f) ? w.at(i) : 0.0;
-  end = run_base + warp_scan(s, lane);
-  above = __ballot_sync(0xffffffffu, s > 0.0 && end > mark), any = __ballot_sync(0xffffffffu, s > 0.0);
-  if (lane == (above ? __ffs(above) - 1 : 31 - __clz(any))) a.out_tokens[row] = i;
+  __syncthreads();
+  if ((int)threadIdx.x != (s_first < kVfThreads ? s_first : s_some)) return;
+  double cum = run - sum;
+  int pick = -1;
+  for (int i = from; i < to; ++i) {
+    const double v = w.at(i);
+    if (v > 0.0) {
+      pick = i;
+      cum += v;
+      if (cum > mark) break;
+    }
+  }
+  a.out_tokens[row] = pick;
 }
 
 template <typename T>
 int launch(const VerifyArgs& a, cudaStream_t st) {
   // Few sequences: 8 CTAs each, for the latency of one row's read. Many: 2 each, which fill the SMs by
   // themselves and exchange less.
-  const int nc = a.batch <= 148 ? kMaxCluster : 2;
+  const int nc = a.batch <= 74 ? 8 : a.batch <= 160 ? 4 : 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.batch * nc);
   cfg.blockDim = dim3(kVfThreads);

@@ -147,6 +147,13 @@ ATTEND = [
     ([(70, 70), (60, 61)], 128, 640, 8, 4, 128),
     ([(2, 2)] * 129, 256, 1000, 2, 1, 64),
     ([(90, 100), (7, 300)], 512, 2200, 3, 1, 128),
+    # sequences with many new rows: causal tiles, ends of the keys inside a tile, several row tiles
+    ([(200, 200), (5, 300), (1, 700)], 16, 0, 3, 1, 128),
+    ([(300, 1000), (2, 1)], 64, 500, 8, 4, 64),
+    ([(40, 9), (7, 130), (0, 50), (30, 30)], 8, 0, 6, 2, 64),  # the first rows of 40 see nothing
+    ([(1, 1), (129, 129), (128, 128), (127, 400)], 32, 77, 2, 2, 128),
+    ([(6, 100)] * 150, 16, 0, 8, 2, 64),  # more items than CTAs
+    ([(5, 70)] * 3 + [(1, 900)] * 20, 16, 0, 16, 1, 128),
 ]
 
 
@@ -259,7 +266,7 @@ def test_attend_bad_pages_hold_no_keys(q4b):
 
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("new,own,g", [(4, 20, 4), (4, 4, 1), (60, 100, 3)])
+@pytest.mark.parametrize("new,own,g", [(4, 20, 4), (4, 4, 1), (60, 100, 3), (150, 290, 2)])
 def test_attend_later_keys_do_not_leak(q4b, value, dtype, new, own, g):
     """A draft whose k or v overflowed spoils its own row and later ones, and no earlier row."""
     for which in (0, 1):
