@@ -7,9 +7,17 @@
 
 namespace q4b {
 
-// first unit of CTA c, and the CTA that holds unit u, for `units` units over `ctas` CTAs
+// First unit of CTA c, and the CTA that holds unit u, for `units` units over `ctas` CTAs.
 __device__ __forceinline__ int cta_first(int c, int units, int ctas) { return (int)((long long)c * units / ctas); }
-__device__ __forceinline__ int cta_of(int u, int units, int ctas) { return (int)((((long long)u + 1) * ctas - 1) / units); }
+// The largest c with cta_first(c) <= u, i.e. with c * units <= (u + 1) * ctas - 1: by a guess in fp32 (off by one at most:
+// c is a few hundred), set right exactly. A 64-bit division would be most of the join's instructions.
+__device__ __forceinline__ int cta_of(int u, int units, int ctas) {
+  const long long n = ((long long)u + 1) * ctas - 1;
+  int c = min((int)__fdividef((float)n, (float)units), ctas - 1);
+  while ((long long)c * units > n) --c;
+  while ((long long)(c + 1) * units <= n) ++c;
+  return c;
+}
 
 // Per sequence, in shared memory; every value bounded.
 struct BatchTable {

@@ -350,6 +350,7 @@ extern "C" int q4b_model_set_trace(q4b_model* model, unsigned long long* events,
 }
 
 extern "C" int q4b_device_status(int reset) {
-  const unsigned v = linear_status(reset != 0) | gemm_status(reset != 0) | prefix_status(reset != 0);
+  const unsigned v = linear_status(reset != 0) | gemm_status(reset != 0) | prefix_tc_status(reset != 0) |
+                     narrow_status(reset != 0);
   return v ? Q4B_ETIMEOUT : Q4B_OK;
 }

@@ -10,22 +10,27 @@
 // items, and at most one cut item at either end): whatever the lengths, every SM streams the same number of
 // bytes. Each run of an item leaves (max, sum, weighted V) in fp32; a last kernel joins a row's parts.
 //
-// Two kernels take items: the tensor-core kernel (prefix_attn_tc.cu) those with many rows, the one here those with
-// few (single tokens, a few drafts) and whatever the other cannot read. Here the tiles of 64 keys come by
-// 16-byte asynchronous copies into a ring of swizzled buffers, STAGES - 1 ahead, the page lookups one tile ahead of
-// the copies; QK and PV are m16n8k16 MMAs on the 16-bit values as stored, fp32 sums, an online softmax in
-// base 2. P is rounded to the cache's type for the PV product: its error, half a step per weight,
-// averages out over the keys and stays below the output's own rounding.
+// Three kernels take items. The tensor-core kernel (prefix_attn_tc.cu) takes those with many rows. Here, with m16n8k16
+// MMAs on the 16-bit values as stored, fp32 sums and an online softmax in base 2:
 //
-// Narrow form (row tiles of 8 or 16): bound by memory, so what counts is few instructions and registers per key. The
-// four warps share a tile's keys (16 each) and hold S^T = K Q^T and O^T = V^T P^T: the keys fill the MMA's 16
-// rows and the 8 columns are the query rows, where S = Q K^T would pad 3 or 4 query rows to 16. P^T moves
-// from S^T's accumulator layout to a B operand by transposing 8 x 8 blocks in registers.
-// Wide form (row tiles of 64): each warp 16 rows against all keys; items of up to 16 rows split the keys instead.
+// Narrow (row tiles of 8 or 16: single tokens, a few drafts): bound by memory, or by the latency of a tile where a
+// CTA has only a few. A producer warp looks the pages up and brings tiles of 64 keys by TMA (a box per page, 128-byte
+// swizzle, a ring of STAGES tiles); four warps share a tile's keys, 16 each, and run free of one another but for
+// the merge at an item's end. They hold S^T = K Q^T and O^T = V^T P^T: the keys fill the MMA's 16 rows and its 8
+// columns are the query rows, where S = Q K^T would pad 3 or 4 query rows to 16. P^T moves from S^T's accumulator
+// layout to a B operand by transposing 8 x 8 blocks in registers. Measured: 192 single tokens behind 180k keys of
+// their own stream at 6.2 TB/s, 0.95 of the copy rate; with 16-byte copies by all threads instead of TMA a tile of
+// keys took 1.5 us of a CTA's time, 0.6 of them for the copies' addresses.
+// Wide (row tiles of 64): whatever the others cannot read (pages of other sizes, head_dim 32). 16-byte asynchronous
+// copies, each warp 16 rows against all keys; items of up to 16 rows split the keys instead.
+//
+// P is rounded to the cache's type for the PV product: its error, half a step per weight, averages out over
+// the keys and stays below the output's own rounding.
 #include <algorithm>
 #include <type_traits>
 
 #include "attn_line.cuh"
+#include "tc.cuh"
 
 namespace q4b {
 namespace {
@@ -34,9 +39,10 @@ constexpr int kThreads = 128;
 constexpr int kRing = 8;  // page lookups in flight (tiles), >= STAGES + 2
 constexpr int kSms = 148;
 constexpr int kMaxBatch = 4096;
-constexpr int kNarrowMaxRows = 128;
 
-template <int HD, int TR>
+__device__ unsigned g_narrow_status = 0;
+
+template <int HD>
 struct Cfg {
   static constexpr int STAGES = HD == 128 ? 3 : 4;
   static constexpr int CTAS = HD == 128 ? 2 : 3;  // per SM
@@ -51,6 +57,9 @@ __device__ __forceinline__ uint32_t sw(int r, int c) {
   if constexpr (HD == 32) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
   return r * (HD * 2) + ((c ^ (r & 7)) << 4);
 }
+
+// the same in the TMA's layout: 64-element (128-byte) halves of the tile one behind the other
+__device__ __forceinline__ uint32_t sw_tma(int r, int c) { return (c >> 3) * (kMmKeys * 128) + r * 128 + (((c ^ r) & 7) << 4); }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -237,10 +246,235 @@ struct Wide {
   }
 };
 
-// ---- narrow form -------------------------------------------------------------------------------------
-
-// column of O^T's element hd of row r in the merge buffer: spreads a warp's stores over the banks
+// column of element hd of row r in the merge buffers: spreads a warp's stores over the banks
 __device__ __forceinline__ int merge_col(int r, int hd) { return hd ^ (((r >> 1) & 3) << 3); }
+
+// For the join: where each row's own item lies. Sequences go round the CTAs. By all threads of the kernel that stands last in
+// front of the join; waits for the kernel in front of it. Uses up the table's running sums.
+template <int TR, int THREADS>
+__device__ __forceinline__ void join_records(const PrefixArgs& a, const BatchTable& table, bool bad, int units, int* scan) {
+  auto records = [&](const AttnLine& l, int first, int tr, bool tc) {
+    for (int b = blockIdx.x; b < a.b.batch; b += gridDim.x) {
+      const int n = table.q0[b + 1] - table.q0[b], mine = table.cum[b + 1] - table.cum[b];
+      if (bad || n * a.g <= l.own_lo || n * a.g > l.own_hi) continue;
+      const int row_tiles = (n * a.g + tr - 1) / tr, tiles = mine / (row_tiles * a.Hkv);
+      for (int j = threadIdx.x; j < n; j += THREADS)
+        a.rec[table.q0[b] + j] = make_int4(first + table.cum[b], tc ? -tiles : tiles, row_tiles, j);
+    }
+  };
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.totals[0] = units;
+  records(a.mm, a.mm.prefix_units, TR, false);
+  for (int t = blockIdx.x * THREADS + threadIdx.x; t < a.rows; t += gridDim.x * THREADS)
+    if (bad || t < table.q0[0] || t >= table.q0[a.b.batch]) a.rec[t] = make_int4(0, 0, 1, -1);
+  if (a.tc_ctas) {
+    __syncthreads();
+    const int own_units = line_table<THREADS, kTcRows, kTcKeys>(a, a.tc, table, bad, scan);
+    records(a.tc, 0, kTcRows, true);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.totals[1] = own_units;
+    griddep_wait();
+  }
+}
+
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_wide_kernel(PrefixArgs a) {
+  using C = Cfg<HD>;
+  constexpr int TR = 64, MERGE = 16;  // MERGE: rows of an item whose warps share the keys
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_koff[kRing][kMmKeys];  // byte offset of a tile's keys in the pools, -1: not there
+  __shared__ unsigned s_mask[kRing][2];
+  __shared__ int s_scan[kThreads / 32];
+  __shared__ float s_m[4][MERGE], s_l[4][MERGE];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  BatchTable table;
+  table.cum = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE);
+  table.q0 = table.cum + a.b.batch + 1;
+  table.len = table.q0 + a.b.batch + 1;
+  // Behind the tensor-core kernel the inputs are there already (it lets this kernel start only behind its own wait), and
+  // its results matter to the join alone, which must find both kernels complete: so the wait comes last.
+  griddep_launch_dependents();
+  if (!a.tc_ctas) griddep_wait();
+  const bool bad = batch_table<kThreads>(a, table);
+  const int units = a.mm.prefix_units + line_table<kThreads, TR, kMmKeys>(a, a.mm, table, bad, s_scan);
+  const Line<TR, kMmKeys> line{a, a.mm, table};
+  const int ctas = min((int)gridDim.x, units);  // fewer units than CTAs: one each, so that no run is empty
+  int u0 = 0, count = 0;
+  if ((int)blockIdx.x < ctas) {
+    u0 = cta_first(blockIdx.x, units, ctas);
+    count = cta_first(blockIdx.x + 1, units, ctas) - u0;
+  }
+
+  const uint32_t s0 = smem_u32(smem);
+  Cursor look = {};
+  if (count) look = line.at(u0);
+  Cursor cur = look;
+
+  // Page lookup of a unit (the `look` cursor stands there): threads 0..63 take a key each. The load is left in flight.
+  struct Lookup {
+    int page, slot, h;
+  };
+  auto lookup = [&]() {
+    Lookup l = {-1, 0, look.h};
+    int key = look.tile * kMmKeys + tid;
+    if (tid < kMmKeys && key < look.limit) {
+      const int pi = key / a.kv.page_size;
+      l.slot = key - pi * a.kv.page_size;
+      l.page = __ldg(look.b < 0 ? a.prefix_pages + pi : a.b.page_table + look.b * a.b.table_stride + pi);
+    }
+    return l;
+  };
+  auto publish = [&](int x, const Lookup& l) {
+    if (tid < kMmKeys) {
+      const bool on = l.page >= 0 && l.page < a.kv.n_pages;
+      s_koff[x % kRing][tid] = on ? 2 * (l.page * a.kv.page_stride + l.slot * a.kv.slot_stride + l.h * a.kv.head_stride) : -1;
+      const unsigned bits = __ballot_sync(0xffffffffu, on);
+      if (lane == 0) s_mask[x % kRing][warp] = bits;
+    }
+  };
+  constexpr int PASS = kThreads / C::CHUNKS;  // tile rows per pass of the CTA's copies, a multiple of 8
+  const int r0 = tid / C::CHUNKS;
+  const uint32_t dst0 = s0 + sw<HD>(r0, tid % C::CHUNKS);
+  const char* k0 = static_cast<const char*>(a.kv.k) + 16 * (tid % C::CHUNKS);
+  const long long kv_gap = static_cast<const char*>(a.kv.v) - static_cast<const char*>(a.kv.k);
+  auto issue = [&](int x) {
+    const uint32_t dst = dst0 + (x % C::STAGES) * C::STAGE;
+#pragma unroll
+    for (int i = 0; i < kMmKeys / PASS; ++i) {
+      const long long off = s_koff[x % kRing][r0 + i * PASS];
+      const bool on = off >= 0;
+      const char* src = k0 + (on ? off : 0);
+      cp16(dst + i * PASS * HD * 2, src, on);
+      cp16(dst + i * PASS * HD * 2 + C::HALF, src + kv_gap, on);
+    }
+  };
+
+  Lookup pend = {-1, 0, 0};
+  {
+    Lookup l[C::STAGES];
+#pragma unroll
+    for (int x = 0; x < C::STAGES; ++x) {
+      if (x < count) l[x] = lookup();
+      if (x + 1 < count) line.next(look);
+    }
+#pragma unroll
+    for (int x = 0; x < C::STAGES; ++x)
+      if (x < count) publish(x, l[x]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < C::STAGES - 1; ++x) {
+    if (x < count) issue(x);
+    cp_commit();
+  }
+
+  Wide<T, HD> w;
+  bool split_keys = false;  // the warps share the tile's keys, not the rows
+  auto start = [&]() {
+    split_keys = cur.nrows <= 16;
+    w.start(a, cur, split_keys ? 0 : warp * 16, lane);
+  };
+  if (count) start();
+  bool began = cur.tile == 0;  // the item's first unit is this CTA's
+  for (int i = 0; i < count; ++i) {
+    cp_wait<C::STAGES - 2>();
+    __syncthreads();
+    if (i + C::STAGES - 1 < count) issue(i + C::STAGES - 1);
+    cp_commit();
+    const bool more = i + C::STAGES < count;
+    if (more) pend = lookup();
+    const bool ends = cur.tile == cur.tiles - 1, run_ends = ends || i + 1 == count;
+
+    const uint32_t ks = s0 + (i % C::STAGES) * C::STAGE, vs = ks + C::HALF;
+    const uint64_t mask = (uint64_t)s_mask[i % kRing][1] << 32 | s_mask[i % kRing][0];
+    const int key0 = cur.tile * kMmKeys;
+    if (mask) {
+      const bool whole = mask == ~0ull && key0 + kMmKeys <= cur.first;
+      bool odd = false;
+      if (cur.first < cur.limit && key0 + kMmKeys > cur.first) {
+        // keys that the first row may not see and the last one does: is any of their V infinite or NaN?
+        constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+        const int lo = max(cur.first - key0, 0);
+        bool found = false;
+        for (int x = tid + lo * C::CHUNKS; x < kMmKeys * C::CHUNKS; x += kThreads) {
+          const uint4 v = *reinterpret_cast<const uint4*>(smem + (vs - s0) + sw<HD>(x / C::CHUNKS, x % C::CHUNKS));
+          const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) found |= (vv[e] & E) == E || (vv[e] >> 16 & E) == E;
+        }
+        odd = __syncthreads_or(found);
+      }
+      if (split_keys)
+        w.template tile<2>(ks, vs, warp * 16, key0, mask, whole, odd, a.scale2, lane);
+      else if (warp * 16 < cur.nrows)
+        w.template tile<8>(ks, vs, 0, key0, mask, whole, odd, a.scale2, lane);
+    }
+    if (more) {
+      publish(i + C::STAGES, pend);
+      if (i + C::STAGES + 1 < count) line.next(look);
+    }
+
+    if (!run_ends) {
+      ++cur.tile;
+      continue;
+    }
+    // the run of this item ends here: its part
+    w.end();
+    const Dest d = dest<TR>(a, cur, began, ends, 0, a.mm_o, a.mm_ml, HD);
+    if (!split_keys) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = warp * 16 + (lane >> 2) + 8 * e;
+        if (r < cur.nrows) {
+          const long long row = d.row(r);
+          float* op = d.o + row * HD + 2 * (lane & 3);
+#pragma unroll
+          for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(op + 8 * n) = make_float2(w.o[n][2 * e], w.o[n][2 * e + 1]);
+          if ((lane & 3) == 0) d.ml[row] = make_float2(w.m[e], w.l[e]);
+        }
+      }
+    } else {
+      // merge the warps' keys in the tile buffer just read ([4][MERGE][HD] fp32 is its size)
+      float* so = reinterpret_cast<float*>(smem + (ks - s0)) + warp * MERGE * HD;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = (lane >> 2) + 8 * e;
+        if (r < cur.nrows) {
+#pragma unroll
+          for (int n = 0; n < HD / 8; ++n)
+            *reinterpret_cast<float2*>(so + r * HD + merge_col(r, 8 * n + 2 * (lane & 3))) = make_float2(w.o[n][2 * e], w.o[n][2 * e + 1]);
+          if ((lane & 3) == 0) s_m[warp][r] = w.m[e], s_l[warp][r] = w.l[e];
+        }
+      }
+      __syncthreads();
+      so = reinterpret_cast<float*>(smem + (ks - s0));
+      for (int x = tid; x < cur.nrows * HD; x += kThreads) {
+        const int r = x / HD, e = x - r * HD;
+        const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        float o = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float f = ex2(s_m[k][r] - ref);
+          o = fmaf(f, so[(k * MERGE + r) * HD + merge_col(r, e)], o);
+          l = fmaf(f, s_l[k][r], l);
+        }
+        const long long row = d.row(r);
+        d.o[row * HD + e] = o;
+        if (e == 0) d.ml[row] = make_float2(mm, l);
+      }
+    }
+    if (i + 1 < count) {
+      line.next_item(cur);
+      began = true;
+      start();
+    }
+  }
+
+  join_records<TR, kThreads>(a, table, bad, units, s_scan);
+}
+
+// ---- narrow form -------------------------------------------------------------------------------------
 
 template <typename T, int HD, int TR>
 struct Narrow {
@@ -250,6 +484,14 @@ struct Narrow {
   float m[NR][2], l[NR][2];  // rows 8 n + 2 (lane % 4) + e
   int lim[NR][2];
 
+  // Asks for the rows of the item to come while the last tile of this one runs: a lane a line of 128 bytes. (Held in registers
+  // instead, they would cost more occupancy than the rest of the loads' latency does.)
+  static __device__ __forceinline__ void ask(const PrefixArgs& a, const Cursor& c, int lane) {
+    constexpr int LINES = HD / 64;
+    const int r = lane / LINES;
+    if (r < min(TR, c.nrows))
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(q_row<T>(a, c, TR, r) + lane % LINES * 64));
+  }
   __device__ __forceinline__ void start(const PrefixArgs& a, const Cursor& c, int lane) {
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
@@ -272,7 +514,8 @@ struct Narrow {
     }
   }
 
-  // the 16 keys from key `k0` of the tile; the other arguments as in the wide form
+  // The 16 keys from key `k0` of the tile. `mask`: the tile's keys that exist; `whole`: all do, for every row.
+  // `odd`: some V that not every row may see is infinite or NaN, so that 0 * v is not 0.
   __device__ __forceinline__ void tile(uint32_t ks, uint32_t vs, int k0, int key0, uint64_t mask, bool whole, bool odd,
                                        float scale2, int lane) {
     float s[NR][4];  // key k0 + lane / 4 + 8 (e / 2), row 8 n + 2 (lane % 4) + e % 2
@@ -284,7 +527,7 @@ struct Narrow {
 #pragma unroll
     for (int k = 0; k < HD / 16; ++k) {
       uint32_t f[4];
-      ldsm4(f, ks + sw<HD>(k0 + (mat & 1) * 8 + mr, 2 * k + (mat >> 1)));
+      ldsm4(f, ks + sw_tma(k0 + (mat & 1) * 8 + mr, 2 * k + (mat >> 1)));
 #pragma unroll
       for (int n = 0; n < NR; ++n) mma<T>(s[n], f, q[k][n][0], q[k][n][1]);
     }
@@ -333,7 +576,7 @@ struct Narrow {
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         uint32_t v[4];
-        ldsm4t(v, vs + sw<HD>(k0 + (mat >> 1) * 8 + mr, 2 * k + (mat & 1)));
+        ldsm4t(v, vs + sw_tma(k0 + (mat >> 1) * 8 + mr, 2 * k + (mat & 1)));
 #pragma unroll
         for (int n = 0; n < NR; ++n) mma<T>(o[k][n], v, p[n][0], p[n][1]);
       }
@@ -352,7 +595,7 @@ struct Narrow {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               unsigned short w;
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(vs + sw<HD>(c, 2 * k + h) + 2 * (lane >> 2)));
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(vs + sw_tma(c, 2 * k + h) + 2 * (lane >> 2)));
               const float v = Half16<T>::unpack(w).x;
               if (see0) o[k][n][2 * h] = fmaf(p0, v, o[k][n][2 * h]);
               if (see1) o[k][n][2 * h + 1] = fmaf(p1, v, o[k][n][2 * h + 1]);
@@ -372,19 +615,31 @@ struct Narrow {
   }
 };
 
-// ---- the kernel --------------------------------------------------------------------------------------
+
+constexpr int kNarrowThreads = 160;  // four warps for the keys and the producer
 
 template <typename T, int HD, int TR>
-__global__ void __launch_bounds__(kThreads, Cfg<HD, TR>::CTAS) prefix_attn_kernel(PrefixArgs a) {
-  using C = Cfg<HD, TR>;
-  constexpr bool WIDE = TR == 64;
-  constexpr int MERGE = WIDE ? 16 : TR;  // rows of an item whose warps share the keys
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long s_koff[kRing][kMmKeys];  // byte offset of a tile's keys in the pools, -1: not there
-  __shared__ unsigned s_mask[kRing][2];
-  __shared__ int s_scan[kThreads / 32];
-  __shared__ float s_m[4][MERGE], s_l[4][MERGE];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+__global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
+    prefix_narrow_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, PrefixArgs a) {
+  using C = Cfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t s0 = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (s0 - smem_u32(smem_raw));
+  __shared__ uint64_t full[C::STAGES], empty[C::STAGES];
+  __shared__ unsigned long long s_mask[C::STAGES];
+  __shared__ int s_scan[kNarrowThreads / 32], s_fail;
+  __shared__ float s_m[4][TR], s_l[4][TR];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 4);
+    }
+    s_fail = 0;
+    fence_mbar_init();
+    tma_prefetch_map(&tk);
+    tma_prefetch_map(&tv);
+  }
   BatchTable table;
   table.cum = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE);
   table.q0 = table.cum + a.b.batch + 1;
@@ -393,8 +648,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, TR>::CTAS) prefix_attn_kerne
   // its results matter to the join alone, which must find both kernels complete: so the wait comes last.
   griddep_launch_dependents();
   if (!a.tc_ctas) griddep_wait();
-  const bool bad = batch_table<kThreads>(a, table);
-  const int units = a.mm.prefix_units + line_table<kThreads, TR, kMmKeys>(a, a.mm, table, bad, s_scan);
+  const bool bad = batch_table<kNarrowThreads>(a, table);
+  const int units = a.mm.prefix_units + line_table<kNarrowThreads, TR, kMmKeys>(a, a.mm, table, bad, s_scan);
   const Line<TR, kMmKeys> line{a, a.mm, table};
   const int ctas = min((int)gridDim.x, units);  // fewer units than CTAs: one each, so that no run is empty
   int u0 = 0, count = 0;
@@ -402,170 +657,127 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, TR>::CTAS) prefix_attn_kerne
     u0 = cta_first(blockIdx.x, units, ctas);
     count = cta_first(blockIdx.x + 1, units, ctas) - u0;
   }
+  volatile int* fail = &s_fail;
 
-  const uint32_t s0 = smem_u32(smem);
-  Cursor look = {};
-  if (count) look = line.at(u0);
-  Cursor cur = look;
-
-  // page lookup of unit x (the `look` cursor stands there): threads 0..63 take a key each
-  long long pend = -1;
-  auto lookup = [&]() {
-    if (tid < kMmKeys) {
-      const int key = look.tile * kMmKeys + tid;
-      pend = -1;
-      if (key < look.limit) {
-        const int pi = key / a.kv.page_size;
-        const int page = __ldg(look.b < 0 ? a.prefix_pages + pi : a.b.page_table + look.b * a.b.table_stride + pi);
-        if (page >= 0 && page < a.kv.n_pages)
-          pend = 2 * (page * a.kv.page_stride + (key - pi * a.kv.page_size) * a.kv.slot_stride + look.h * a.kv.head_stride);
-      }
-    }
-  };
-  auto publish = [&](int x) {
-    if (tid < kMmKeys) {
-      s_koff[x % kRing][tid] = pend;
-      const unsigned bits = __ballot_sync(0xffffffffu, pend >= 0);
-      if (lane == 0) s_mask[x % kRing][warp] = bits;
-    }
-  };
-  constexpr int PASS = kThreads / C::CHUNKS;  // tile rows per pass of the CTA's copies, a multiple of 8
-  const int r0 = tid / C::CHUNKS;
-  const uint32_t dst0 = s0 + sw<HD>(r0, tid % C::CHUNKS);
-  const char* k0 = static_cast<const char*>(a.kv.k) + 16 * (tid % C::CHUNKS);
-  const long long kv_gap = static_cast<const char*>(a.kv.v) - static_cast<const char*>(a.kv.k);
-  auto issue = [&](int x) {
-    const uint32_t dst = dst0 + (x % C::STAGES) * C::STAGE;
-#pragma unroll
-    for (int i = 0; i < kMmKeys / PASS; ++i) {
-      const long long off = s_koff[x % kRing][r0 + i * PASS];
-      const bool on = off >= 0;
-      const char* src = k0 + (on ? off : 0);
-      cp16(dst + i * PASS * HD * 2, src, on);
-      cp16(dst + i * PASS * HD * 2 + C::HALF, src + kv_gap, on);
-    }
-  };
-
-  for (int x = 0; x < C::STAGES && x < count; ++x) {
-    lookup();
-    publish(x);
-    if (x + 1 < count) line.next(look);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int x = 0; x < C::STAGES - 1; ++x) {
-    if (x < count) issue(x);
-    cp_commit();
-  }
-
-  typename std::conditional<WIDE, Wide<T, HD>, Narrow<T, HD, WIDE ? 8 : TR>>::type w;
-  bool split_keys = !WIDE;  // the warps share the tile's keys, not the rows
-  auto start = [&]() {
-    if constexpr (WIDE) {
-      split_keys = cur.nrows <= 16;
-      w.start(a, cur, split_keys ? 0 : warp * 16, lane);
-    } else {
-      w.start(a, cur, lane);
-    }
-  };
-  if (count) start();
-  bool began = cur.tile == 0;  // the item's first unit is this CTA's
-  for (int i = 0; i < count; ++i) {
-    cp_wait<C::STAGES - 2>();
-    __syncthreads();
-    if (i + C::STAGES - 1 < count) issue(i + C::STAGES - 1);
-    cp_commit();
-    const bool more = i + C::STAGES < count;
-    if (more) lookup();
-
-    const uint32_t ks = s0 + (i % C::STAGES) * C::STAGE, vs = ks + C::HALF;
-    const uint64_t mask = (uint64_t)s_mask[i % kRing][1] << 32 | s_mask[i % kRing][0];
-    const int key0 = cur.tile * kMmKeys;
-    if (mask) {
-      const bool whole = mask == ~0ull && key0 + kMmKeys <= cur.first;
-      bool odd = false;
-      if (cur.first < cur.limit && key0 + kMmKeys > cur.first) {
-        // keys that the first row may not see and the last one does: is any of their V infinite or NaN?
-        constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-        const int lo = max(cur.first - key0, 0);
-        bool found = false;
-        for (int x = tid + lo * C::CHUNKS; x < kMmKeys * C::CHUNKS; x += kThreads) {
-          const uint4 v = *reinterpret_cast<const uint4*>(smem + (vs - s0) + sw<HD>(x / C::CHUNKS, x % C::CHUNKS));
-          const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) found |= (vv[e] & E) == E || (vv[e] >> 16 & E) == E;
-        }
-        odd = __syncthreads_or(found);
-      }
-      if constexpr (WIDE) {
-        if (split_keys)
-          w.template tile<2>(ks, vs, warp * 16, key0, mask, whole, odd, a.scale2, lane);
-        else if (warp * 16 < cur.nrows)
-          w.template tile<8>(ks, vs, 0, key0, mask, whole, odd, a.scale2, lane);
-      } else {
-        w.tile(ks, vs, warp * 16, key0, mask, whole, odd, a.scale2, lane);
-      }
-    }
-    if (more) {
-      publish(i + C::STAGES);
-      if (i + C::STAGES + 1 < count) line.next(look);
-    }
-
-    const bool ends = cur.tile == cur.tiles - 1;
-    if (!ends && i + 1 < count) {
-      ++cur.tile;
-      continue;
-    }
-    // the run of this item ends here: its part
-    w.end();
-    const Dest d = dest<TR>(a, cur, began, ends, 0, a.mm_o, a.mm_ml, HD);
-    if (!split_keys) {
-      if constexpr (WIDE) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = warp * 16 + (lane >> 2) + 8 * e;
-          if (r < cur.nrows) {
-            const long long row = d.row(r);
-            float* op = d.o + row * HD + 2 * (lane & 3);
-#pragma unroll
-            for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(op + 8 * n) = make_float2(w.o[n][2 * e], w.o[n][2 * e + 1]);
-            if ((lane & 3) == 0) d.ml[row] = make_float2(w.m[e], w.l[e]);
-          }
+  if (warp == 4 && count) {
+    // producer: lane l brings box l of each tile; its page is looked up one tile ahead
+    const int box = min(a.kv.page_size, kMmKeys), boxes = kMmKeys / box;
+    Cursor c = line.at(u0);
+    auto page_of = [&]() {
+      int page = -1;
+      const int key = c.tile * kMmKeys + lane * box;
+      if (lane < boxes && key < c.limit)
+        page = __ldg((c.b < 0 ? a.prefix_pages : a.b.page_table + c.b * a.b.table_stride) + key / a.kv.page_size);
+      return page;
+    };
+    int page = page_of(), issued = 0;
+    for (int i = 0; i < count; ++i) {
+      const int s = i % C::STAGES, key = c.tile * kMmKeys + lane * box, left = c.limit - key, h = c.h;
+      const bool there = page >= 0 && page < a.kv.n_pages;  // lanes without a box or with no key left: not
+      unsigned long long mask = 0;
+      if (there) mask = (left >= 64 ? ~0ull : (1ull << left) - 1) & (box == 64 ? ~0ull : (1ull << box) - 1);
+      mask <<= (lane * box) & 63;
+      unsigned lo = __reduce_or_sync(0xffffffffu, (unsigned)mask), hi = __reduce_or_sync(0xffffffffu, (unsigned)(mask >> 32));
+      bool ok = true;
+      if (lane == 0) {
+        ok = i < C::STAGES || mbar_wait_bounded(&empty[s], (i / C::STAGES - 1) & 1, kWaitLimitNs);
+        if (ok) {
+          s_mask[s] = (unsigned long long)hi << 32 | lo;
+          mbar_arrive_expect_tx(&full[s], C::STAGE);
+        } else {
+          *fail = 1;
         }
       }
-    } else {
-      // merge the warps' keys in the tile buffer just read ([4][MERGE][HD] fp32 is at most its size)
-      float* so = reinterpret_cast<float*>(smem + (ks - s0)) + warp * MERGE * HD;
-      __syncthreads();
-      if constexpr (WIDE) {
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (lane < boxes) {  // a page out of the pool reads as zeros
+        const uint32_t dst = s0 + s * C::STAGE + lane * box * 128;
+        const int slot = key % a.kv.page_size, from = there ? page : a.kv.n_pages;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = (lane >> 2) + 8 * e;
-          if (r < cur.nrows) {
-#pragma unroll
-            for (int n = 0; n < HD / 8; ++n)
-              *reinterpret_cast<float2*>(so + r * HD + merge_col(r, 8 * n + 2 * (lane & 3))) = make_float2(w.o[n][2 * e], w.o[n][2 * e + 1]);
-            if ((lane & 3) == 0) s_m[warp][r] = w.m[e], s_l[warp][r] = w.l[e];
-          }
+        for (int x = 0; x < HD / 64; ++x) {
+          tma_load_4d(dst + x * kMmKeys * 128, &tk, 64 * x, slot, h, from, &full[s]);
+          tma_load_4d(dst + C::HALF + x * kMmKeys * 128, &tv, 64 * x, slot, h, from, &full[s]);
         }
-      } else {
+      }
+      issued = i + 1;
+      if (issued < count) {
+        line.next(c);
+        page = page_of();
+      }
+    }
+    if (lane == 0 && *fail)  // leave no copy in flight
+      for (int i = max(issued - C::STAGES, 0); i < issued; ++i) mbar_wait_bounded(&full[i % C::STAGES], (i / C::STAGES) & 1, kWaitLimitNs);
+  } else if (warp < 4 && count) {
+    Cursor cur = line.at(u0);
+    Narrow<T, HD, TR> w;
+    w.start(a, cur, lane);
+    bool began = cur.tile == 0;  // the item's first unit is this CTA's
+    for (int i = 0; i < count; ++i) {
+      const bool ends = cur.tile == cur.tiles - 1, run_ends = ends || i + 1 == count;
+      Cursor next = cur;
+      if (ends && i + 1 < count) {
+        line.next_item(next);
+        w.ask(a, next, lane);
+      }
+      const int s = i % C::STAGES, key0 = cur.tile * kMmKeys;
+      // After a wait that gave up, the run goes on without waiting (the warps meet at barriers), to no use.
+      if (!*fail && !mbar_wait_bounded(&full[s], (i / C::STAGES) & 1, kWaitLimitNs)) *fail = 1;
+      __syncwarp();
+      const uint32_t ks = s0 + s * C::STAGE, vs = ks + C::HALF;
+      const unsigned long long mask = s_mask[s];
+      const int k0 = warp * 16;
+      bool wrote = false;
+      if ((mask >> k0) & 0xffff) {
+        bool odd = false;
+        if (key0 + k0 + 16 > cur.first) {
+          // Keys that the first row does not see: V of those that no row sees becomes zero (a page's rest holds anything);
+          // is any of the others' infinite or NaN?
+          constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+          bool found = false;
+          for (int x = lane; x < 16 * C::CHUNKS; x += 32) {
+            const int key = k0 + x / C::CHUNKS;
+            uint4* v = reinterpret_cast<uint4*>(smem + (vs - s0) + sw_tma(key, x % C::CHUNKS));
+            if (key0 + key >= cur.limit) {
+              *v = make_uint4(0, 0, 0, 0);
+            } else if (key0 + key >= cur.first) {
+              const uint4 old = *v;
+              const uint32_t vv[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
-        for (int n = 0; n < TR / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = 8 * n + 2 * (lane & 3) + e;
-            if (r < cur.nrows) {
-#pragma unroll
-              for (int k = 0; k < HD / 16; ++k)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) so[r * HD + merge_col(r, 16 * k + 8 * h + (lane >> 2))] = w.o[k][n][2 * h + e];
-              if (lane < 4) s_m[warp][r] = w.m[n][e], s_l[warp][r] = w.l[n][e];
+              for (int e = 0; e < 4; ++e) found |= (vv[e] & E) == E || (vv[e] >> 16 & E) == E;
             }
           }
+          odd = __any_sync(0xffffffffu, found);
+          wrote = true;
+        }
+        w.tile(ks, vs, k0, key0, mask, mask == ~0ull && key0 + kMmKeys <= cur.first, odd, a.scale2, lane);
       }
-      __syncthreads();
-      so = reinterpret_cast<float*>(smem + (ks - s0));
-      for (int x = tid; x < cur.nrows * HD; x += kThreads) {
+      if (!run_ends) {
+        if (wrote) fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+        ++cur.tile;
+        continue;
+      }
+      // The run of this item ends here: merge the warps' keys in the tile buffer just read ([4][TR][HD] fp32 is at most
+      // its size), and write the part.
+      w.end();
+      const Dest d = dest<TR>(a, cur, began, ends, 0, a.mm_o, a.mm_ml, HD);
+      float* so = reinterpret_cast<float*>(smem + (ks - s0));
+      named_bar_sync(1, 128);
+#pragma unroll
+      for (int n = 0; n < TR / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 8 * n + 2 * (lane & 3) + e;
+          if (r < cur.nrows) {
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) so[(warp * TR + r) * HD + merge_col(r, 16 * k + 8 * x + (lane >> 2))] = w.o[k][n][2 * x + e];
+            if (lane < 4) s_m[warp][r] = w.m[n][e], s_l[warp][r] = w.l[n][e];
+          }
+        }
+      named_bar_sync(1, 128);
+      for (int x = threadIdx.x; x < cur.nrows * HD; x += 128) {
         const int r = x / HD, e = x - r * HD;
         const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
         const float ref = mm == -INFINITY ? 0.0f : mm;
@@ -573,43 +785,27 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, TR>::CTAS) prefix_attn_kerne
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float f = ex2(s_m[k][r] - ref);
-          o = fmaf(f, so[(k * MERGE + r) * HD + merge_col(r, e)], o);
+          o = fmaf(f, so[(k * TR + r) * HD + merge_col(r, e)], o);
           l = fmaf(f, s_l[k][r], l);
         }
         const long long row = d.row(r);
         d.o[row * HD + e] = o;
-        if (e == 0) d.ml[row] = make_float2(mm, l);
+        // a row whose work gave up is NaN
+        if (e == 0) d.ml[row] = make_float2(mm, *fail ? __int_as_float(0x7fffffff) : l);
+      }
+      if (i + 1 < count) {
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+        cur = next;
+        began = true;
+        w.start(a, cur, lane);
       }
     }
-    if (i + 1 < count) {
-      line.next_item(cur);
-      began = true;
-      start();
-    }
   }
-
-  // For the join: where each row's own item lies. Sequences go round the CTAs.
-  if (blockIdx.x == 0 && tid == 0) a.totals[0] = units;
-  auto records = [&](const AttnLine& l, const BatchTable& t, int prefix_units, int tr, int tk, bool tc) {
-    for (int b = blockIdx.x; b < a.b.batch; b += gridDim.x) {
-      const int n = t.q0[b + 1] - t.q0[b], mine = t.cum[b + 1] - t.cum[b];
-      const bool here = n * a.g > l.own_lo && n * a.g <= l.own_hi;
-      if (!here || bad) continue;
-      const int row_tiles = (n * a.g + tr - 1) / tr, tiles = mine / (row_tiles * a.Hkv);
-      for (int j = tid; j < n; j += kThreads)
-        a.rec[t.q0[b] + j] = make_int4(prefix_units + t.cum[b], tc ? -tiles : tiles, row_tiles, j);
-    }
-  };
-  records(a.mm, table, a.mm.prefix_units, TR, kMmKeys, false);
-  for (int t = blockIdx.x * kThreads + tid; t < a.rows; t += gridDim.x * kThreads)
-    if (bad || t < table.q0[0] || t >= table.q0[a.b.batch]) a.rec[t] = make_int4(0, 0, 1, -1);
-  if (a.tc_ctas) {
-    __syncthreads();
-    const int own_units = line_table<kThreads, kTcRows, kTcKeys>(a, a.tc, table, bad, s_scan);
-    records(a.tc, table, 0, kTcRows, kTcKeys, true);
-    if (blockIdx.x == 0 && tid == 0) a.totals[1] = own_units;
-    griddep_wait();
-  }
+  __syncthreads();
+  if (threadIdx.x == 0 && *fail) atomicOr(&g_narrow_status, kStatusTimeout);
+  join_records<TR, kNarrowThreads>(a, table, bad, units, s_scan);
 }
 
 // Joins a row's parts, half a warp per (row, head): every part is (max, sum, weighted V); the prefix's and the own
@@ -622,11 +818,11 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixArgs a)
   constexpr int E = HD / 16;
   const int lane = threadIdx.x & 15;
   const unsigned half = 0xffffu << (threadIdx.x & 16);
-  const long long row = ((long long)blockIdx.x * kJoinThreads + threadIdx.x) / 16;
+  const int row = (blockIdx.x * kJoinThreads + threadIdx.x) / 16, n_rows = a.rows * a.H;  // at most 10^8
   griddep_launch_dependents();
   griddep_wait();
-  if (row >= (long long)a.rows * a.H) return;
-  const int t = (int)(row / a.H), head = (int)(row - (long long)t * a.H), h = head / a.g;
+  if (row >= n_rows) return;
+  const int t = row / a.H, head = row - t * a.H, h = head / a.g;
   const int4 rec = __ldcg(a.rec + t);
   const int mm_units = __ldcg(a.totals), tc_own_units = a.tc_ctas ? __ldcg(a.totals + 1) : 0;
   if (rec.w < 0) return;  // a row of no sequence
@@ -640,12 +836,14 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixArgs a)
   auto find = [&](bool tc, bool pre, int first, int row_tiles, int tiles, int j) {
     Item it;
     it.cut0 = tc && !pre ? a.tc_ctas : 0;
-    it.tr = tc ? kTcRows : a.mm_rows;
+    const int shift = tc ? 8 : a.mm_rows == 8 ? 3 : a.mm_rows == 16 ? 4 : 6;
+    static_assert(kTcRows == 1 << 8, "the shift above");
+    it.tr = 1 << shift;
     it.ml = tc ? a.tc_ml : a.mm_ml;
     it.o = tc ? a.tc_o : a.mm_o;
     const int units = !tc ? mm_units : pre ? a.tc.prefix_units : tc_own_units, ctas = min(tc ? a.tc_ctas : a.mm_ctas, units);
-    const int rr = j * a.g + head - h * a.g, rt = rr / it.tr;
-    it.r = rr - rt * it.tr;
+    const int rr = j * a.g + head - h * a.g, rt = rr >> shift;
+    it.r = rr - (rt << shift);
     it.c0 = it.n = 0;
     if (tiles > 0) {
       const int u = first + (h * row_tiles + rt) * tiles;
@@ -670,7 +868,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixArgs a)
       const bool first = k0 + lane < pre.n;
       const Item& it = first ? pre : own;
       const int k = k0 + lane - (first ? 0 : pre.n);
-      const long long at = it.n == 1 ? row + (first ? 0 : (long long)a.rows * a.H)
+      const long long at = it.n == 1 ? row + (first ? 0ll : (long long)n_rows)
                                      : (2ll * (it.cut0 + it.c0 + k) + (k == 0)) * it.tr + it.r;
       x = __ldcg((it.n == 1 ? a.row_ml : it.ml) + at);
       o = (it.n == 1 ? a.row_o : it.o) + at * HD;
@@ -710,7 +908,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixArgs a)
     }
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no keys: zero
-  T* out = static_cast<T*>(a.out) + row * HD;
+  T* out = static_cast<T*>(a.out) + (long long)row * HD;
   if constexpr (E >= 4) {
 #pragma unroll
     for (int q = 0; q < E / 4; ++q)
@@ -723,7 +921,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixArgs a)
 
 // ---- host --------------------------------------------------------------------------------------------
 
-int mm_ctas_per_sm(int hd) { return hd == 128 ? Cfg<128, 64>::CTAS : hd == 64 ? Cfg<64, 64>::CTAS : Cfg<32, 64>::CTAS; }
+int mm_ctas_per_sm(int hd) { return hd == 128 ? Cfg<128>::CTAS : hd == 64 ? Cfg<64>::CTAS : Cfg<32>::CTAS; }
 
 // Which kernel takes what; decided by what the host knows, so that a captured graph keeps its launches.
 struct Plan {
@@ -748,10 +946,10 @@ Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv, bool wide
   p.tc.own_lo = tc_own ? kTcMinRows : kAll;
   p.tc.own_hi = kAll;
   p.mm.own_hi = tc_own ? kTcMinRows : kAll;
-  // Row tiles: the narrow form up to a few of them (their keys come from L2 again), else the wide one.
+  // Row tiles: 8 for single tokens, 16 for a few rows; more rows are more tiles, whose keys come from L2 again.
   const bool prefix_here = !tc_prefix && b.prefix_len > 0;
-  const int most = std::max(tc_own ? std::min(R, kTcMinRows) : rows > b.batch ? R : g, prefix_here ? R : 0);
-  p.mm_rows = most <= 8 ? 8 : most <= kNarrowMaxRows ? 16 : 64;
+  const int most = std::max(rows > b.batch ? R : g, prefix_here ? R : 0);
+  p.mm_rows = !prefix_tc_takes(kv) ? 64 : most <= 8 ? 8 : 16;
   if (prefix_here) p.mm.prefix_units = prefix_units(rows, g, Hkv, b.prefix_len, p.mm_rows, kMmKeys);
   p.mm_ctas = mm_ctas_per_sm(kv.head_dim) * kSms;
   return p;
@@ -783,19 +981,40 @@ Layout layout(const Plan& p, int rows, int H, int hd) {
   return w;
 }
 
-template <typename T, int HD, int TR>
-cudaError_t launch_mm(const PrefixArgs& a, cudaStream_t st) {
-  using C = Cfg<HD, TR>;
-  auto kern = prefix_attn_kernel<T, HD, TR>;
+size_t table_bytes(int batch) { return 12 * ((size_t)batch + 1); }
+
+template <typename T, int HD>
+cudaError_t launch_wide(const PrefixArgs& a, cudaStream_t st) {
+  using C = Cfg<HD>;
+  auto kern = prefix_wide_kernel<T, HD>;
   static std::atomic<unsigned long long> done;
-  const cudaError_t e = set_max_dynamic_smem(kern, C::STAGES * C::STAGE + 12 * (kMaxBatch + 1), done);
+  const cudaError_t e = set_max_dynamic_smem(kern, C::STAGES * C::STAGE + (int)table_bytes(kMaxBatch), done);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kern, dim3(a.mm_ctas), dim3(kThreads), C::STAGES * C::STAGE + 12 * (a.b.batch + 1), st, a);
+  return launch_pdl(kern, dim3(a.mm_ctas), dim3(kThreads), C::STAGES * C::STAGE + table_bytes(a.b.batch), st, a);
+}
+
+template <typename T, int HD, int TR>
+cudaError_t launch_narrow(const PrefixArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+  using C = Cfg<HD>;
+  auto kern = prefix_narrow_kernel<T, HD, TR>;
+  static std::atomic<unsigned long long> done;
+  const cudaError_t e = set_max_dynamic_smem(kern, C::STAGES * C::STAGE + 1024 + (int)table_bytes(kMaxBatch), done);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, dim3(a.mm_ctas), dim3(kNarrowThreads), C::STAGES * C::STAGE + 1024 + table_bytes(a.b.batch), st, tk, tv, a);
 }
 
 template <typename T, int HD>
 int launch(const PrefixArgs& a, cudaStream_t st) {
-  cudaError_t e = a.mm_rows == 8 ? launch_mm<T, HD, 8>(a, st) : a.mm_rows == 16 ? launch_mm<T, HD, 16>(a, st) : launch_mm<T, HD, 64>(a, st);
+  cudaError_t e = cudaSuccess;
+  if (a.mm_rows == 64) {
+    e = launch_wide<T, HD>(a, st);
+  } else if constexpr (HD >= 64) {
+    CUtensorMap tk, tv;
+    const int box = std::min(a.kv.page_size, kMmKeys);
+    if (int rc = make_tmap_pages(&tk, a.kv, a.kv.k, box)) return rc;
+    if (int rc = make_tmap_pages(&tv, a.kv, a.kv.v, box)) return rc;
+    e = a.mm_rows == 8 ? launch_narrow<T, HD, 8>(a, tk, tv, st) : launch_narrow<T, HD, 16>(a, tk, tv, st);
+  }
   if (e == cudaSuccess)
     e = launch_pdl(prefix_join_kernel<T, HD>, dim3((unsigned)(((long long)a.rows * a.H * 16 + kJoinThreads - 1) / kJoinThreads)),
                    dim3(kJoinThreads), 0, st, a);
@@ -823,6 +1042,17 @@ int check(const char* what, int rows, int n_heads, const q4b_batch* b, const q4b
 }
 
 }  // namespace
+
+unsigned narrow_status(bool reset) {
+  unsigned v = 0;
+  cudaMemcpyFromSymbol(&v, g_narrow_status, sizeof(v));
+  if (reset && v) {
+    const unsigned zero = 0;
+    cudaMemcpyToSymbol(g_narrow_status, &zero, sizeof(zero));
+  }
+  return v;
+}
+
 }  // namespace q4b
 
 using namespace q4b;

@@ -23,7 +23,7 @@ struct PrefixArgs {
   void* out;  // [rows, H * hd]
   int tc_ctas;       // CTAs of the tensor-core kernel, 0: not launched
   int mm_ctas;       // CTAs of the mma.sync kernel
-  int mm_rows;       // its rows per row tile
+  int mm_rows;       // its rows per row tile: 8 or 16 (narrow), 64 (wide)
   AttnLine tc, mm;
   int4* rec;         // [rows]: where the join finds a row's own item (see RowRec)
   int* totals;       // units of the mm line, own units of the tc line
@@ -41,9 +41,10 @@ constexpr int kTcMaxBatch = 2048;  // the sequences' table shares the tensor-cor
 constexpr int kTcMinUnits = 5000;  // prefix tiles of 16 rows x 64 keys from which the tensor-core kernel pays off
 constexpr int kTcMinRows = 64;     // rows x heads of a sequence from which it takes the own keys
 
-// whether the tensor-core kernel can read this cache
+// whether the kernels that load by TMA can read this cache
 bool prefix_tc_takes(const q4b_paged_kv& kv);
 int prefix_tc_run(const PrefixArgs& a, cudaStream_t st);
-unsigned prefix_status(bool reset);
+unsigned prefix_tc_status(bool reset);
+unsigned narrow_status(bool reset);
 
 }  // namespace q4b

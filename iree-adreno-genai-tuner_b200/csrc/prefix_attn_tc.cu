@@ -48,14 +48,6 @@ struct TcCfg {
   static constexpr int SMEM = (2 + SLOTS) * TILE + 1024;   // + alignment to the swizzle's 1024 bytes
 };
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
-
 // D[tmem] (+)= A[tmem] * B[smem]
 __device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                               uint32_t accumulate) {
@@ -607,7 +599,7 @@ int prefix_tc_run(const PrefixArgs& a, cudaStream_t st) {
   return h16 ? launch<__half, 64>(a, st) : launch<__nv_bfloat16, 64>(a, st);
 }
 
-unsigned prefix_status(bool reset) {
+unsigned prefix_tc_status(bool reset) {
   unsigned v = 0;
   cudaMemcpyFromSymbol(&v, g_prefix_status, sizeof(v));
   if (reset && v) {
