@@ -518,18 +518,18 @@ struct Narrow {
   // `odd`: some V that not every row may see is infinite or NaN, so that 0 * v is not 0.
   __device__ __forceinline__ void tile(uint32_t ks, uint32_t vs, int k0, int key0, uint64_t mask, bool whole, bool odd,
                                        float scale2, int lane) {
-    float s[NR][4];  // key k0 + lane / 4 + 8 (e / 2), row 8 n + 2 (lane % 4) + e % 2
+    float s[NR][4], s2[NR][4];  // key k0 + lane / 4 + 8 (e / 2), row 8 n + 2 (lane % 4) + e % 2; two chains of sums
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.0f;
     const int mat = lane >> 3, mr = lane & 7;
 #pragma unroll
     for (int k = 0; k < HD / 16; ++k) {
       uint32_t f[4];
       ldsm4(f, ks + sw_tma(k0 + (mat & 1) * 8 + mr, 2 * k + (mat >> 1)));
 #pragma unroll
-      for (int n = 0; n < NR; ++n) mma<T>(s[n], f, q[k][n][0], q[k][n][1]);
+      for (int n = 0; n < NR; ++n) mma<T>(k & 1 ? s2[n] : s[n], f, q[k][n][0], q[k][n][1]);
     }
     bool moved = false;
     float f[NR][2];
@@ -537,7 +537,7 @@ struct Narrow {
     for (int n = 0; n < NR; ++n) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] *= scale2;
+        s[n][e] = (s[n][e] + s2[n][e]) * scale2;
         if (!whole) {
           const int c = k0 + (lane >> 2) + 8 * (e >> 1);
           if (!((mask >> c) & 1) || key0 + c >= lim[n][e & 1]) s[n][e] = -INFINITY;
@@ -748,7 +748,8 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
           odd = __any_sync(0xffffffffu, found);
           wrote = true;
         }
-        w.tile(ks, vs, k0, key0, mask, mask == ~0ull && key0 + kMmKeys <= cur.first, odd, a.scale2, lane);
+        const bool whole = mask == ~0ull && key0 + kMmKeys <= cur.first;
+        w.tile(ks, vs, k0, key0, mask, whole, odd, a.scale2, lane);
       }
       if (!run_ends) {
         if (wrote) fence_async_smem();
@@ -777,19 +778,24 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
           }
         }
       named_bar_sync(1, 128);
-      for (int x = threadIdx.x; x < cur.nrows * HD; x += 128) {
-        const int r = x / HD, e = x - r * HD;
+      // HD / 4 lanes a row, four elements each
+      constexpr int LANES = HD / 4;
+#pragma unroll 2
+      for (int r = threadIdx.x / LANES; r < cur.nrows; r += 128 / LANES) {
+        const int e = threadIdx.x % LANES * 4;
         const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
         const float ref = mm == -INFINITY ? 0.0f : mm;
-        float o = 0.0f, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float f = ex2(s_m[k][r] - ref);
-          o = fmaf(f, so[(k * TR + r) * HD + merge_col(r, e)], o);
+          const float4 v = *reinterpret_cast<const float4*>(so + (k * TR + r) * HD + merge_col(r, e));
+          o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
           l = fmaf(f, s_l[k][r], l);
         }
         const long long row = d.row(r);
-        d.o[row * HD + e] = o;
+        *reinterpret_cast<float4*>(d.o + row * HD + e) = o;
         // a row whose work gave up is NaN
         if (e == 0) d.ml[row] = make_float2(mm, *fail ? __int_as_float(0x7fffffff) : l);
       }

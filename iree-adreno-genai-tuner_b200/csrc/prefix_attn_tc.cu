@@ -44,8 +44,8 @@ struct TcCfg {
   static constexpr int HALVES = HD / 64;                   // 64-column (128-byte) halves of a row
   static constexpr int ATOM = kTcKeys * 128;               // one half of a 128-row tile, bytes
   static constexpr int TILE = HALVES * ATOM;               // Q half, K or V tile
-  static constexpr int SLOTS = HD == 128 ? 4 : 8;          // K and V tiles in flight
-  static constexpr int SMEM = (2 + SLOTS) * TILE + 1024;   // + alignment to the swizzle's 1024 bytes
+  static constexpr int SLOTS = HD == 128 ? 2 : 4;          // pairs of a V and the next K tile in flight
+  static constexpr int SMEM = (2 + 2 * SLOTS) * TILE + 1024;  // + alignment to the swizzle's 1024 bytes
 };
 
 // D[tmem] (+)= A[tmem] * B[smem]
@@ -167,6 +167,33 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t v) {
   return (v & (H16 ? 0x7C007C00u : 0x7F807F80u)) + (H16 ? 0x04000400u : 0x00800080u);
 }
 
+// pairs of fp32 in one instruction
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, PrefixArgs a) {
@@ -202,7 +229,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   griddep_wait();
   griddep_launch_dependents();  // behind the wait: what runs next may read the inputs at once
   BatchTable table;
-  table.cum = reinterpret_cast<int*>(smem + (2 + C::SLOTS) * C::TILE);
+  table.cum = reinterpret_cast<int*>(smem + (2 + 2 * C::SLOTS) * C::TILE);
   table.q0 = table.cum + a.b.batch + 1;
   table.len = table.q0 + a.b.batch + 1;
   int own_units = 0;
@@ -224,12 +251,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == 8) {
-      // producer: entry x of the ring is K (even) or V (odd) of the run's key tile x / 2
+      // producer: an item's run of n tiles is n + 1 entries of the ring, entry p its V tile p - 1 and K tile p: what one round of
+      // the MMA thread needs, under one barrier
       const int box = min(a.kv.page_size, kTcKeys), boxes = kTcKeys / box;
       int x = 0;
       bool ok = true;
       for (Segs g(line, run_own, run_prefix); ok && g.valid(); g.next()) {
         const Seg& s = g.s;
+        const int n = s.n();
+        if (n == 0) continue;
         const int32_t* pages = page_row(a, s.c);
         auto page_of = [&](int j) {
           int page = a.kv.n_pages;  // out of the map: zeros
@@ -240,30 +270,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           return page;
         };
-        int page = s.n() ? page_of(s.t0) : 0;
-        for (int j = s.t0; ok && j < s.e1; ++j) {
-          int next = 0;
-          for (int v = 0; ok && v < 2; ++v, ++x) {
-            const int slot = x % C::SLOTS, r = x / C::SLOTS;
-            if (lane == 0) {
-              ok = r == 0 || mbar_wait_bounded(&empty[slot], (r - 1) & 1, kWaitLimitNs);
-              if (ok) {
-                mbar_arrive_expect_tx(&full[slot], C::TILE);
-                s_issued = x + 1;
-              } else {
-                *fail = 1;
-              }
-            }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (!ok) break;
-            if (v == 0 && j + 1 < s.e1) next = page_of(j + 1);
-            if (lane < boxes) {
-              const int at = (j * kTcKeys + lane * box) % a.kv.page_size;
-              const uint32_t dst = base + (2 + slot) * C::TILE + lane * box * 128;
-  #pragma unroll
-              for (int c = 0; c < C::HALVES; ++c) tma_load_4d(dst + c * C::ATOM, v ? &tv : &tk, 64 * c, at, s.c.h, page, &full[slot]);
+        int page = page_of(s.t0), before = 0;  // of K tile p, of V tile p - 1
+        for (int p = 0; p <= n; ++p, ++x) {
+          const int slot = x % C::SLOTS, r = x / C::SLOTS, j = s.t0 + p;
+          if (lane == 0) {
+            ok = r == 0 || mbar_wait_bounded(&empty[slot], (r - 1) & 1, kWaitLimitNs);
+            if (ok) {
+              mbar_arrive_expect_tx(&full[slot], p == 0 || p == n ? C::TILE : 2 * C::TILE);
+              s_issued = x + 1;
+            } else {
+              *fail = 1;
             }
           }
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) break;
+          const int next = p + 1 < n ? page_of(j + 1) : 0;
+          if (lane < boxes) {
+            const uint32_t dst = base + (2 + 2 * slot) * C::TILE + lane * box * 128;
+            const int key = j * kTcKeys + lane * box;
+#pragma unroll
+            for (int c = 0; c < C::HALVES; ++c) {
+              if (p < n) tma_load_4d(dst + c * C::ATOM, &tk, 64 * c, key % a.kv.page_size, s.c.h, page, &full[slot]);
+              if (p > 0) tma_load_4d(dst + C::TILE + c * C::ATOM, &tv, 64 * c, (key - kTcKeys) % a.kv.page_size, s.c.h, before, &full[slot]);
+            }
+          }
+          before = page;
           page = next;
         }
       }
@@ -273,23 +304,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         constexpr uint32_t bf = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
         constexpr uint32_t idesc_s = idesc_f16_f32(kHalf, kTcKeys, false, false) | bf;
         constexpr uint32_t idesc_o = idesc_f16_f32(kHalf, HD, false, true) | bf;
-        auto slot = [&](int x) { return base + (2 + x % C::SLOTS) * C::TILE; };
+        // Descriptors are made once and moved by adding to their address field (16-byte units): made anew for each MMA they
+        // were most of this thread's time, and this thread was what the kernel waited for.
+        const uint64_t q_desc = sw128_desc(base, 16, 1024), k_desc = sw128_desc(base + 2 * C::TILE, 16, 1024),
+                       v_desc = sw128_desc(base + 3 * C::TILE, C::ATOM, 1024);
         auto wait_full = [&](int x) { return mbar_wait_bounded(&full[x % C::SLOTS], (x / C::SLOTS) & 1, kWaitLimitNs); };
         auto qk = [&](int i, int x) {
-          const uint32_t q = base + i * C::TILE, k = slot(x);
-  #pragma unroll
+          const uint64_t q = q_desc + i * (C::TILE >> 4), k = k_desc + x % C::SLOTS * (2 * C::TILE >> 4);
+#pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (kk / 4) * C::ATOM + (kk % 4) * 32;
-            tc_mma_f16(tmem + kS + 128 * i, sw128_desc(q + off, 16, 1024), sw128_desc(k + off, 16, 1024), idesc_s, kk != 0);
+            const int off = ((kk / 4) * C::ATOM + (kk % 4) * 32) >> 4;
+            tc_mma_f16(tmem + kS + 128 * i, q + off, k + off, idesc_s, kk != 0);
           }
           tc_commit(&s_full[i]);
         };
         auto pv = [&](int i, int x, bool first) {
-          const uint32_t v = slot(x);
-  #pragma unroll
+          const uint64_t v = v_desc + x % C::SLOTS * (2 * C::TILE >> 4);
+#pragma unroll
           for (int kk = 0; kk < kTcKeys / 16; ++kk)
-            tc_mma_f16_ta(tmem + kO + HD * i, tmem + kS + 128 * i + 8 * kk, sw128_desc(v + kk * 2048, C::ATOM, 1024),
-                          idesc_o, !(first && kk == 0));
+            tc_mma_f16_ta(tmem + kO + HD * i, tmem + kS + 128 * i + 8 * kk, v + (kk * 2048 >> 4), idesc_o, !(first && kk == 0));
         };
         int x = 0, items = 0, items1 = 0, tiles = 0, tiles1 = 0;  // so far; ...1: those with a second half
         bool ok = true;
@@ -305,25 +338,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           if (ok) tc_commit(&empty[x % C::SLOTS]);
           for (int j = 0; ok && j < n; ++j) {
-            const int xv = x + 2 * j + 1, xk = xv + 1;
-            ok = wait_full(xv);
+            ++x;
+            ok = wait_full(x);
             for (int i = 0; ok && i < active; ++i) {
               ok = mbar_wait_bounded(&p_full[i], ((i ? tiles1 : tiles) + j) & 1, kWaitLimitNs);
-              if (ok && i == 0 && j + 1 < n) ok = wait_full(xk);
               if (!ok) break;
               tc_fence_after();
-              pv(i, xv, j == 0);
+              pv(i, x, j == 0);
               if (j + 1 < n)
-                qk(i, xk);
+                qk(i, x);
               else
                 tc_commit(&o_full[i]);
             }
-            if (ok) {
-              tc_commit(&empty[xv % C::SLOTS]);
-              if (j + 1 < n) tc_commit(&empty[xk % C::SLOTS]);
-            }
+            if (ok) tc_commit(&empty[x % C::SLOTS]);
           }
-          x += 2 * n;
+          ++x;
           tiles += n, ++items;
           if (active == 2) tiles1 += n, ++items1;
         }
@@ -372,7 +401,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int n = s.n();
       g.next();
       if (i >= s.active()) {
-        x += 2 * n;
+        if (n > 0) x += n + 1;
         if (g.valid()) load_q(g.s);
         continue;
       }
@@ -387,7 +416,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const unsigned there = __ballot_sync(0xffffffffu, page >= 0 && page < a.kv.n_pages);
         const bool edge = key0 + kTcKeys > s.c.first;  // some row does not see all of the tile's keys
         if (edge) {
-          const int xv = x + 2 * j + 1;
+          const int xv = x + j + 1;
           ok = mbar_wait_bounded(&full[xv % C::SLOTS], (xv / C::SLOTS) & 1, kWaitLimitNs);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
@@ -396,7 +425,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // V of the keys that not every row sees: zeros behind the last one, and over what is not finite
           constexpr int ROW = 8 * C::HALVES;  // 16-byte chunks of a row
           const int from = max(s.c.first - key0, 0), to = min(s.c.limit - key0, kTcKeys);
-          uint8_t* v = smem + (2 + xv % C::SLOTS) * C::TILE;
+          uint8_t* v = smem + (3 + 2 * (xv % C::SLOTS)) * C::TILE;
           auto chunk = [&](int y) { return reinterpret_cast<uint4*>(v + (y % ROW / 8) * C::ATOM + y / ROW * 128 + (y % 8) * 16); };
           uint32_t odd = 0;
 #pragma unroll 4
@@ -452,7 +481,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = 0; c < 4; ++c) {
           mx[c] = __uint_as_float(sc[c][0]);
 #pragma unroll
-          for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(sc[c][e]));
+          for (int e = 1; e < 31; e += 2) mx[c] = max3(mx[c], __uint_as_float(sc[c][e]), __uint_as_float(sc[c][e + 1]));
+          mx[c] = fmaxf(mx[c], __uint_as_float(sc[c][31]));
         }
         const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         const float top = best * a.scale2;
@@ -473,20 +503,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t scale = pair(a.scale2, a.scale2), off = pair(-ref, -ref);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {  // P's 16 columns lie over columns of S that have been read
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float y0 = ex2(fmaf(__uint_as_float(sc[c][2 * e]), a.scale2, -ref));
-            const float y1 = ex2(fmaf(__uint_as_float(sc[c][2 * e + 1]), a.scale2, -ref));
-            sum[e & 3] += y0 + y1;
-            p[e] = Half16<T>::pack(y0, y1);
+            float2 y = unpair(fma2(pair(__uint_as_float(sc[c][2 * e]), __uint_as_float(sc[c][2 * e + 1])), scale, off));
+            y.x = ex2(y.x);
+            y.y = ex2(y.y);
+            sum[e & 1] = add2(sum[e & 1], pair(y.x, y.y));
+            p[e] = Half16<T>::pack(y.x, y.y);
           }
           tmem_st_16(ts + 16 * c, p);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float2 s01 = unpair(add2(sum[0], sum[1]));
+        l += s01.x + s01.y;
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_full[i]);
@@ -540,9 +573,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (on) d.ml[at] = make_float2(m, l);
       tc_fence_before();  // O has been read: the next item's first PV waits for this half's P
-      x += 2 * n;
       tiles += n;
-      if (n > 0) ++items;
+      if (n > 0) x += n + 1, ++items;
     }
   }
   tc_fence_before();
