@@ -850,8 +850,9 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixArgs a)
     const int units = !tc ? mm_units : pre ? a.tc.prefix_units : tc_own_units, ctas = min(tc ? a.tc_ctas : a.mm_ctas, units);
     const int rr = j * a.g + head - h * a.g, rt = rr >> shift;
     it.r = rr - (rt << shift);
-    it.c0 = it.n = 0;
-    if (tiles > 0) {
+    it.c0 = 0;
+    it.n = tiles > 0;
+    if (tiles > (tc && !pre ? kTcWholeTiles : 0)) {
       const int u = first + (h * row_tiles + rt) * tiles;
       it.c0 = cta_of(u, units, ctas);
       it.n = cta_of(u + tiles - 1, units, ctas) - it.c0 + 1;

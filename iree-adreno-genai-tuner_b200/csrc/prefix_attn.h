@@ -36,6 +36,7 @@ struct PrefixArgs {
 };
 
 constexpr int kTcRows = 256, kTcKeys = 128, kTcCtas = 148;
+constexpr int kTcWholeTiles = 8;  // own items of up to so many tiles are not cut between CTAs
 constexpr int kMmKeys = 64;
 constexpr int kTcMaxBatch = 2048;  // the sequences' table shares the tensor-core kernel's shared memory
 constexpr int kTcMinUnits = 5000;  // prefix tiles of 16 rows x 64 keys from which the tensor-core kernel pays off

@@ -242,11 +242,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t tmem = s_tmem;
   volatile int* fail = &s_fail;
   const Line<kTcRows, kTcKeys> line{a, a.tc, table};
-  auto share = [&](int units, int first) {
-    const int ctas = min((int)gridDim.x, units), c = blockIdx.x;  // fewer units than CTAs: one each, no run is empty
-    return c < ctas ? make_int2(first + cta_first(c, units, ctas), first + cta_first(c + 1, units, ctas)) : make_int2(0, 0);
+  const int cta = blockIdx.x;
+  auto share = [&](int units) {
+    const int ctas = min((int)gridDim.x, units);  // fewer units than CTAs: one each, no run is empty
+    return cta < ctas ? make_int2(cta_first(cta, units, ctas), cta_first(cta + 1, units, ctas)) : make_int2(0, 0);
   };
-  const int2 run_own = share(own_units, a.tc.prefix_units), run_prefix = share(a.tc.prefix_units, 0);
+  // A run of own keys begins and ends between items where the item is short: an item's start and end cost about as much as
+  // two or three tiles, and another part for the join.
+  auto whole = [&](int u) {
+    if (u == 0 || u == own_units) return u;
+    const Cursor c = line.at(a.tc.prefix_units + u);
+    return c.tiles > kTcWholeTiles ? u : u - c.tile + (2 * c.tile < c.tiles ? 0 : c.tiles);
+  };
+  int2 run_own = share(own_units);
+  run_own = make_int2(a.tc.prefix_units + whole(run_own.x), a.tc.prefix_units + whole(run_own.y));
+  const int2 run_prefix = share(a.tc.prefix_units);
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
