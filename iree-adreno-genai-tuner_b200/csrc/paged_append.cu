@@ -19,6 +19,7 @@ int check_batch(const char* what, const q4b_batch* b, int rows) {
   if (!b) return set_error(Q4B_EINVAL, "%s: null batch", what);
   if (rows < 0 || b->batch < 0 || b->table_width < 0 || b->prefix_len < 0)
     return set_error(Q4B_EINVAL, "%s: negative size", what);
+  if (b->prefix_len > 0x7fffff00) return set_error(Q4B_EINVAL, "%s: prefix_len %d is too large", what, b->prefix_len);
   if (!b->q_start || (b->batch > 0 && !b->seq_lens) || (b->batch > 0 && b->table_width > 0 && !b->page_table))
     return set_error(Q4B_EINVAL, "%s: null batch array", what);
   if (b->batch > 1 && b->table_stride < b->table_width)
@@ -211,6 +212,9 @@ extern "C" int q4b_paged_rope_append(const void* q, const void* k, const void* v
   if (int rc = check_batch(what, batch, rows)) return rc;
   if (int rc = check_paged_kv(what, kv)) return rc;
   if (!q || !k || !v || !q_out) return set_error(Q4B_EINVAL, "%s: null pointer", what);
+  if ((kv->n_pages > 1 && kv->page_stride == 0) || (kv->page_size > 1 && kv->slot_stride == 0) ||
+      (kv->n_kv_heads > 1 && kv->head_stride == 0))
+    return set_error(Q4B_EINVAL, "%s: the cache's slots overlap (a stride of zero)", what);
   if (x_dtype != Q4B_F32 && x_dtype != kv->dtype)
     return set_error(Q4B_EINVAL, "%s: q, k and v are fp32 or of the cache's type", what);
   if (n_heads < 1) return set_error(Q4B_EINVAL, "%s: n_heads < 1", what);

@@ -49,6 +49,8 @@ APPEND_BAD = [
     ({}, {}, dict(slot_stride=68), b"strides"),
     ({}, {}, dict(k=8), b"aligned"),
     ({}, {}, dict(n_pages=0), b"empty"),
+    ({}, {}, dict(slot_stride=0), b"overlap"),
+    ({}, {}, dict(page_stride=0), b"overlap"),
 ]
 
 
@@ -64,6 +66,43 @@ def test_append_refuses(L, args, batch, kv, word):
                                  ctypes.byref(c), a["out"], None)
     assert rc == _lib.Q4B_EINVAL
     assert word in L.q4b_last_error(), L.q4b_last_error()
+
+
+ATTEND_BAD = [
+    (dict(q=None), {}, {}, b"null"), (dict(out=None), {}, {}, b"null"),
+    (dict(pages=None), dict(prefix_len=5), {}, b"null"), (dict(qs=511), {}, {}, b"even strides"),
+    (dict(q=18), {}, {}, b"aligned"), (dict(out=8), {}, {}, b"aligned"), (dict(scale=0.0), {}, {}, b"scale"),
+    (dict(scale=float("nan")), {}, {}, b"scale"), (dict(scale=float("inf")), {}, {}, b"scale"),
+    (dict(ws=None), {}, {}, b"workspace"), (dict(ws=4096 + 16), {}, {}, b"workspace"), (dict(wsb=-1), {}, {}, b"workspace"),
+    (dict(heads=3), {}, {}, b"n_kv_heads"), (dict(heads=0), {}, {}, b"n_kv_heads"), (dict(rows=-1), {}, {}, b"negative"),
+    ({}, dict(batch=-1), {}, b"negative"), ({}, dict(q_start=None), {}, b"null"),
+    ({}, dict(prefix_len=2**31 - 1), {}, b"prefix_len"), ({}, {}, dict(dtype=7), b"fp16 or bf16"), ({}, {}, dict(v=24), b"aligned"),
+    ({}, {}, dict(page_stride=-8), b"strides"),
+]
+
+
+@pytest.mark.parametrize("args,batch,kv,word", ATTEND_BAD)
+def test_attention_refuses(L, args, batch, kv, word):
+    from q4b import _lib
+    a = dict(q=16, qs=512, hs=64, rows=3, heads=8, scale=0.125, pages=16, out=16, ws=4096, wsb=0)
+    a.update(args)
+    b, c = _batch(_lib, **batch), _kv(_lib, **kv)
+    need = L.q4b_prefix_attention_workspace(a["rows"], a["heads"], ctypes.byref(b), ctypes.byref(c))
+    rc = L.q4b_prefix_attention(a["q"], a["qs"], a["hs"], a["rows"], a["heads"], a["scale"], a["pages"],
+                                ctypes.byref(b), ctypes.byref(c), a["out"], a["ws"], max(need + a["wsb"], 0), None)
+    assert rc == _lib.Q4B_EINVAL
+    assert word in L.q4b_last_error(), L.q4b_last_error()
+
+
+@pytest.mark.parametrize("rows,batch,kv", [(3, {}, dict(head_dim=48)), (3, dict(batch=5000), {}),
+                                           (20_000_000, {}, {}), (3, dict(table_width=2**30, table_stride=2**30), dict(page_size=64))])
+def test_attention_names_what_it_does_not_handle(L, rows, batch, kv):
+    """Valid calls beyond the kernels' bounds: no workspace size, and an error of their own."""
+    from q4b import _lib
+    b, c = _batch(_lib, **batch), _kv(_lib, **kv)
+    assert L.q4b_prefix_attention_workspace(rows, 8, ctypes.byref(b), ctypes.byref(c)) == 0
+    rc = L.q4b_prefix_attention(16, 512, 64, rows, 8, 0.125, 16, ctypes.byref(b), ctypes.byref(c), 16, 4096, 1 << 40, None)
+    assert rc == _lib.Q4B_EUNSUPPORTED
 
 
 VERIFY_BAD = [
@@ -94,6 +133,8 @@ def test_wrappers_refuse_cpu_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         q4b.paged_rope_append(x, x, x, p, p, t[None], t, torch.zeros(2, dtype=torch.int32))
     with pytest.raises(ValueError, match="CUDA"):
+        q4b.prefix_attention(x, p, p, t, 0, t[None], t, torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="CUDA"):
         q4b.verify_drafts(torch.zeros(1, 8), None, t, torch.zeros(1), torch.zeros(2, dtype=torch.int32))
 
 
@@ -103,6 +144,7 @@ def test_empty_calls_launch_nothing(L):
     assert L.q4b_paged_rope_append(16, 16, 16, 1, 512, 128, 128, 3, 8, 16, 16, 32, 64, 64, 0, ctypes.byref(b),
                                    ctypes.byref(c), 16, None) == 0
     assert L.q4b_verify_drafts(16, 16, 0, 100, 100, 100, 16, 16, 4, 16, 0, 16, 16, None) == 0
+    assert L.q4b_prefix_attention(16, 512, 64, 3, 8, 0.125, None, ctypes.byref(b), ctypes.byref(c), 16, None, 0, None) == 0
 
 
 def test_plain_forms_agree_with_hand_made_values():

@@ -154,6 +154,16 @@ ATTEND = [
     ([(1, 1), (129, 129), (128, 128), (127, 400)], 32, 77, 2, 2, 128),
     ([(6, 100)] * 150, 16, 0, 8, 2, 64),  # more items than CTAs
     ([(5, 70)] * 3 + [(1, 900)] * 20, 16, 0, 16, 1, 128),
+    # prefixes long enough for the tensor-core kernel (more than 5000 tiles of 16 rows x 64 keys): single tokens and
+    # several rows, ends inside a tile, pages smaller and larger than one
+    ([(1, 5)] * 150, 16, 4500, 8, 4, 64),
+    ([(3, 9), (80, 90)], 32, 6000, 16, 4, 128),
+    ([(1, 1)] * 129, 8, 3000, 16, 8, 64),
+    ([(2, 40)] * 100, 256, 3500, 8, 8, 128),
+    ([(1, 0)] * 40, 128, 12800, 8, 8, 64),  # no own keys; 40 rows; whole tiles
+    # many rows from pages that no TMA box fits
+    ([(70, 200), (1, 90)], 20, 333, 3, 1, 128),
+    ([(40, 100)] * 3, 1, 65, 4, 2, 64),
 ]
 
 
@@ -224,22 +234,23 @@ def test_attend_leaves_padding_rows(q4b):
 @pytest.mark.parametrize("hd", [64, 128])
 def test_attend_bad_prefix_pages_hold_no_keys(q4b, hd, dtype):
     """The same where the prefix runs in tiles: single pages, a whole tile and the first tile missing."""
-    case = _attend_case([(20, 70), (30, 40), (1, 8)], 16, 1000, 8, 4, hd, dtype, 5)
-    for i in list(range(8)) + [13] + list(range(24, 32)) + [40, 62]:
-        case[0]["prefix_pages"][i] = -1 if i % 2 else 2**31 - 1
-    _run_attend(q4b, case, 16)
-    case[0]["prefix_pages"][:] = 10**6
-    _run_attend(q4b, case, 16)
+    for prefix, H, Hkv in ((1000, 8, 4), (6000, 16, 8)):
+        case = _attend_case([(20, 70), (30, 40), (1, 8)], 16, prefix, H, Hkv, hd, dtype, 5)
+        for i in list(range(8)) + [13] + list(range(24, 32)) + [40, 62]:
+            case[0]["prefix_pages"][i] = -1 if i % 2 else 2**31 - 1
+        _run_attend(q4b, case, 16)
+        case[0]["prefix_pages"][:] = 10**6
+        _run_attend(q4b, case, 16)
 
 
 def test_attend_growing_scores(q4b):
     """Keys ordered by score, so that the running maximum grows from tile to tile, by little and by much."""
-    for step in (0.02, 2.0):
-        b, q, kp, vp = _attend_case([(1, 9)] * 40, 16, 1024, 4, 2, 64, torch.float16, 5)
+    for step, n, heads in ((0.02, 1024, 2), (2.0, 1024, 2), (0.02, 8192, 8), (2.0, 8192, 8)):
+        b, q, kp, vp = _attend_case([(1, 9)] * 80, 16, n, heads, heads, 64, torch.float16, 5)
         q[:] = 0
         q[:, :, 0] = 1.0
         pages = torch.from_numpy(b["prefix_pages"]).long().to(DEV)
-        kp[pages, :, :, 0] = (torch.arange(1024, device=DEV).view(64, 16, 1) * step).half()
+        kp[pages, :, :, 0] = (torch.arange(n, device=DEV).view(-1, 16, 1) * step).half()
         _run_attend(q4b, (b, q, kp, vp), 16, scale=0.4)
 
 
@@ -266,19 +277,20 @@ def test_attend_bad_pages_hold_no_keys(q4b):
 
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("new,own,g", [(4, 20, 4), (4, 4, 1), (60, 100, 3), (150, 290, 2)])
-def test_attend_later_keys_do_not_leak(q4b, value, dtype, new, own, g):
+@pytest.mark.parametrize("new,own,g,page", [(4, 20, 4, 8), (4, 4, 1, 8), (60, 100, 3, 8), (150, 290, 2, 8), (4, 20, 4, 20),
+                                            (60, 100, 3, 20)])
+def test_attend_later_keys_do_not_leak(q4b, value, dtype, new, own, g, page):
     """A draft whose k or v overflowed spoils its own row and later ones, and no earlier row."""
     for which in (0, 1):
-        case = _attend_case([(new, own), (2, 9)], 8, 30, 2 * g, 2, 64, dtype, 7)
+        case = _attend_case([(new, own), (2, 9)], page, 30, 2 * g, 2, 64, dtype, 7)
         b, q, kp, vp = case
         bad = own - new + 2  # key of row 2
-        (kp, vp)[which][b["page_table"][0, bad // 8], bad % 8] = value
+        (kp, vp)[which][b["page_table"][0, bad // page], bad % page] = value
         d = _dev(b)
         out = _f64(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 30, d["page_table"], d["seq_lens"], d["q_start"]))
         clean = [t for t in range(b["rows"]) if t < 2 or t >= new]
         with np.errstate(all="ignore"):
-            ref = R.attention(_f64(q), _f64(kp), _f64(vp), b, 8).reshape(out.shape)
+            ref = R.attention(_f64(q), _f64(kp), _f64(vp), b, page).reshape(out.shape)
         live = np.zeros(b["rows"], dtype=bool)
         live[clean] = True
         _check_attend(np.where(live[:, None], out, 0), np.where(live[:, None], ref, 0), _f64(vp), dtype, live)
@@ -306,12 +318,13 @@ def test_attend_sharp_scores(q4b):
     _run_attend(q4b, _attend_case([(20, 300), (10, 31)], 16, 700, 8, 2, 64, torch.float16, 9, sharp=3.0), 16, scale=2.0)
 
 
-def test_attend_far_pages(q4b):
+@pytest.mark.parametrize("new", [2, 40])
+def test_attend_far_pages(q4b, new):
     """Element offsets behind 2^32 in the pool."""
     n_pages, page, Hkv, hd = 70_000, 64, 8, 128  # 4.6e9 elements, 9 GB each
     kp = torch.empty(n_pages, page, Hkv, hd, dtype=torch.float16, device=DEV)
     vp = torch.empty_like(kp)
-    b = R.make_batch([(2, 150)], page, 6, prefix_len=100)
+    b = R.make_batch([(new, 150)], page, 6, prefix_len=100)
     far = np.array([69_999, 3, 65_537, 40_000, 68_000, 66_000])
     for name in ("page_table", "prefix_pages"):
         b[name] = far[b[name]].astype(np.int32)
@@ -319,17 +332,17 @@ def test_attend_far_pages(q4b):
     small_k, small_v = (torch.randn(6, page, Hkv, hd, generator=g, device=DEV).half() for _ in range(2))
     at = torch.from_numpy(far).to(DEV)
     kp[at], vp[at] = small_k, small_v
-    q = torch.randn(2, 16, hd, generator=g, device=DEV).half()
+    q = torch.randn(new, 16, hd, generator=g, device=DEV).half()
     d = _dev(b)
     out = _f64(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 100, d["page_table"], d["seq_lens"], d["q_start"]))
     back = {int(x): i for i, x in enumerate(far)}
     b2 = dict(b, page_table=np.vectorize(back.get)(b["page_table"]), prefix_pages=np.vectorize(back.get)(b["prefix_pages"]))
     ref = R.attention(_f64(q), _f64(small_k), _f64(small_v), b2, page)
-    _check_attend(out.reshape(ref.shape), ref, _f64(small_v), torch.float16, np.ones(2, dtype=bool))
+    _check_attend(out.reshape(ref.shape), ref, _f64(small_v), torch.float16, np.ones(new, dtype=bool))
     # and the append reaches them
-    x = torch.randn(2, 2 * Hkv, hd, device=DEV).half()
+    x = torch.randn(new, 2 * Hkv, hd, device=DEV).half()
     q4b.paged_rope_append(q, x[:, :Hkv], x[:, Hkv:], kp, vp, d["page_table"], d["seq_lens"], d["q_start"], prefix_len=100)
-    for j, s in enumerate((148, 149)):
+    for j, s in enumerate(range(150 - new, 150)):
         page_id = int(b["page_table"][0, s // page])
         assert torch.equal(kp[page_id, s % page], x[j, :Hkv]) and torch.equal(vp[page_id, s % page], x[j, Hkv:])
     del kp, vp
