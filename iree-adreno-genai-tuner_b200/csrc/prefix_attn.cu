@@ -960,15 +960,18 @@ Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv, bool wide
   if (prefix_here) p.mm.prefix_units = prefix_units(rows, g, Hkv, b.prefix_len, p.mm_rows, kMmKeys);
   int mm_sms = kSms;
   // Small steps, where either kernel's start and end (some 10 us of launch, first reads and last parts) weigh as much as
-  // its tiles: each on half of the SMs, at once, instead of one behind the other. By the measured time of a CTA's tile
-  // and a guess at the own keys (0.6 of what the page tables hold). 61 sequences of 5 drafts behind 4099 keys:
-  // 45.5 us against 51.7; 192 single tokens behind 16384 keys: 227 against 210, so those stay one behind the other.
+  // its tiles: both at once, the SMs shared by the measured time of their tiles and a guess at the own keys (0.6 of what
+  // the page tables hold), instead of one behind the other. 61 sequences of 5 drafts behind 4099 keys: 45 us against 52;
+  // 192 single tokens behind 16384 keys, where a wrong guess costs more than the start: 207 at best against 210.
   const int per_sequence = (R + std::max(b.batch, 1) - 1) / std::max(b.batch, 1);
   if (tc_prefix && per_sequence <= kTcMinRows && p.mm_rows < 64) {
     const double tc_us = p.tc.prefix_units / (double)kSms * (kv.head_dim == 128 ? 2.0 : 1.4);
     const double mm_us = (double)b.batch * Hkv * ((per_sequence + p.mm_rows - 1) / p.mm_rows) *
                          (0.6 * b.table_width * kv.page_size / kMmKeys) / (mm_ctas_per_sm(kv.head_dim) * kSms) * 1.3;
-    if (2 * std::max(tc_us, mm_us) < 10 + tc_us + mm_us) p.tc_ctas = mm_sms = kSms / 2;
+    if (tc_us + mm_us < 40) {
+      p.tc_ctas = std::min(std::max((int)(kSms * tc_us / (tc_us + mm_us)), kSms / 6), kSms * 3 / 4);
+      mm_sms = kSms - p.tc_ctas;
+    }
   }
   p.mm_ctas = mm_ctas_per_sm(kv.head_dim) * mm_sms;
   return p;

@@ -39,7 +39,9 @@ constexpr int kTcRows = 256, kTcKeys = 128, kTcCtas = 148;
 constexpr int kTcWholeTiles = 8;  // own items of up to so many tiles are not cut between CTAs
 constexpr int kMmKeys = 64;
 constexpr int kTcMaxBatch = 2048;  // the sequences' table shares the tensor-core kernel's shared memory
-constexpr int kTcMinUnits = 5000;  // prefix tiles of 16 rows x 64 keys from which the tensor-core kernel pays off
+// Prefix tiles of 16 rows x 64 keys from which the tensor-core kernel pays off. 32 rows of 3 heads behind 512 keys (384
+// tiles): 25.2 us without it, 25.4 with; behind 2048 (1536 tiles): 32.6 and 28.7.
+constexpr int kTcMinUnits = 500;
 constexpr int kTcMinRows = 64;     // rows x heads of a sequence from which it takes the own keys
 
 // whether the kernels that load by TMA can read this cache

@@ -425,7 +425,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (key0 + 4 * lane < s.c.limit) page = __ldg(pages + (key0 + 4 * lane) / a.kv.page_size);
         const unsigned there = __ballot_sync(0xffffffffu, page >= 0 && page < a.kv.n_pages);
         const bool edge = key0 + kTcKeys > s.c.first;  // some row does not see all of the tile's keys
+        ok = mbar_wait_bounded(&s_full[i], (tiles + j) & 1, kWaitLimitNs);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
         if (edge) {
+          // Behind the wait for S: a half that sat out items may be ahead of the ring by more than the one phase that a
+          // barrier's parity tells apart, but this tile's K is there, so its V is the barrier's current phase.
           const int xv = x + j + 1;
           ok = mbar_wait_bounded(&full[xv % C::SLOTS], (xv / C::SLOTS) & 1, kWaitLimitNs);
           if (!__all_sync(0xffffffffu, ok)) {
@@ -459,11 +466,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
           fence_async_smem();
-        }
-        ok = mbar_wait_bounded(&s_full[i], (tiles + j) & 1, kWaitLimitNs);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
         }
         tc_fence_after();
         uint32_t sc[4][32];

@@ -120,10 +120,10 @@ struct Row {
   }
 };
 
-// A lane's share of the weights of vectors [lo, hi), every 32nd; four 16-byte loads in flight.
+// A lane's share of the weights of vectors [lo, hi), every 32nd; four or eight 16-byte loads in flight.
 template <typename T, bool REST>
 __device__ __forceinline__ double lane_sum(const Weights<T>& w, int head, int lo, int hi, int lane) {
-  constexpr int N = 16 / sizeof(T), U = REST ? 2 : 4;
+  constexpr int N = 16 / sizeof(T), U = 4;
   const T* p = w.p + head;
   const T* d = REST ? w.d + head : nullptr;
   Sum2 sum;
@@ -177,8 +177,12 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
   return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kVfThreads, 5) verify_kernel(VerifyArgs a) {
+// CTAs that an SM holds: registers for p's and d's loads in flight, or p's alone.
+template <bool DRAFT>
+constexpr int kResident = DRAFT ? 4 : 5;
+
+template <typename T, bool DRAFT>
+__global__ void __launch_bounds__(kVfThreads, kResident<DRAFT>) verify_kernel(VerifyArgs a) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -208,7 +212,7 @@ __global__ void __launch_bounds__(kVfThreads, 5) verify_kernel(VerifyArgs a) {
         ok = false;
         if (x >= 0 && x < a.vocab) {
           const float p = prob(as_float(static_cast<const T*>(a.target)[row * a.target_stride + x]));
-          const float d = a.draft ? prob(as_float(static_cast<const T*>(a.draft)[row * a.draft_stride + x])) : 1.0f;
+          const float d = DRAFT ? prob(as_float(static_cast<const T*>(a.draft)[row * a.draft_stride + x])) : 1.0f;
           ok = (double)__ldg(a.uniforms + row) * (double)d < (double)p;
         }
       }
@@ -230,8 +234,8 @@ __global__ void __launch_bounds__(kVfThreads, 5) verify_kernel(VerifyArgs a) {
   const bool cut = kept < n - 1;
   Weights<T> w;
   w.p = static_cast<const T*>(a.target) + row * a.target_stride;
-  w.d = cut && a.draft ? static_cast<const T*>(a.draft) + row * a.draft_stride : nullptr;
-  w.skip = cut && !a.draft ? __ldg(a.tokens + row + 1) : -1;
+  w.d = DRAFT && cut ? static_cast<const T*>(a.draft) + row * a.draft_stride : nullptr;
+  w.skip = !DRAFT && cut ? __ldg(a.tokens + row + 1) : -1;
 
   const int pieces = nc * kVfWarps, piece = rank * kVfWarps + warp;
   double total = 0.0, before = 0.0;  // before: of the pieces in front of this lane's two
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(kVfThreads, 5) verify_kernel(VerifyArgs a) {
     int lo = row_of.value(piece), hi = row_of.value(piece + 1);
     if (row_of.vectors) {
       const int v0 = row_of.vector(piece), v1 = row_of.vector(piece + 1), h = row_of.head;
-      s = w.d ? lane_sum<T, true>(w, h, v0, v1, lane) : lane_sum<T, false>(w, h, v0, v1, lane);
+      s = DRAFT && w.d ? lane_sum<T, true>(w, h, v0, v1, lane) : lane_sum<T, false>(w, h, v0, v1, lane);
       // the values outside vectors: at most N - 1 in front and behind
       if (lo + lane < h + v0 * Row<T>::N) s += w.at(lo + lane);
       if (h + v1 * Row<T>::N + lane < hi) s += w.at(h + v1 * Row<T>::N + lane);
@@ -326,11 +330,12 @@ __global__ void __launch_bounds__(kVfThreads, 5) verify_kernel(VerifyArgs a) {
   a.out_tokens[row] = pick;
 }
 
-template <typename T>
+template <typename T, bool DRAFT>
 int launch(const VerifyArgs& a, cudaStream_t st) {
-  // Few sequences: 8 CTAs each, for the latency of one row's read. Many: 2 each, which fill the SMs by
-  // themselves and exchange less.
-  const int nc = a.batch <= 74 ? 8 : a.batch <= 160 ? 4 : 2;
+  // As many CTAs for each sequence as the SMs hold at once (a second wave for a few of them took half of the time again), 2 at
+  // least.
+  const int slots = 148 * kResident<DRAFT>;
+  const int nc = a.batch * 8ll <= slots ? 8 : a.batch * 4ll <= slots ? 4 : 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.batch * nc);
   cfg.blockDim = dim3(kVfThreads);
@@ -343,7 +348,7 @@ int launch(const VerifyArgs& a, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel<T>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel<T, DRAFT>, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(Q4B_ELAUNCH, "verify_drafts: launch failed: %s", cudaGetErrorString(e));
@@ -380,6 +385,7 @@ extern "C" int q4b_verify_drafts(const void* target, const void* draft, int dtyp
   a.tokens = tokens, a.q_start = q_start, a.uniforms = uniforms;
   a.out_tokens = out_tokens, a.accepted = accepted;
   const cudaStream_t st = as_stream(stream);
-  if (dtype == Q4B_F32) return launch<float>(a, st);
-  return dtype == Q4B_F16 ? launch<__half>(a, st) : launch<__nv_bfloat16>(a, st);
+  if (dtype == Q4B_F32) return draft ? launch<float, true>(a, st) : launch<float, false>(a, st);
+  if (dtype == Q4B_F16) return draft ? launch<__half, true>(a, st) : launch<__half, false>(a, st);
+  return draft ? launch<__nv_bfloat16, true>(a, st) : launch<__nv_bfloat16, false>(a, st);
 }
