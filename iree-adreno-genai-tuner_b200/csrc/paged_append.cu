@@ -8,7 +8,9 @@
 // through L1 by the token's heads). A task is 16 elements of one head: both sides of eight pairs, so that
 // every access is 16 or 32 bytes. A CTA takes `tok` tokens: first each token's place (sequence, page, slot,
 // position) is found by one warp, then all threads walk the tasks. Few tokens get one CTA each (latency),
-// many share CTAs so that the searches are paid once per 8 tokens.
+// many share CTAs so that the searches are paid once per 8 tokens. Measured: 13,375 rows of 32 + 2 * 8 heads of 128 in
+// bf16 (336 MB) 59 us, 5.7 TB/s, 0.87 of the copy rate; one token 3.6 us, which is the launch. Stepping through the
+// tasks without divisions, 16-byte table loads and four tokens a CTA changed nothing or cost time (58-67 us).
 #include <algorithm>
 
 #include "paged.cuh"

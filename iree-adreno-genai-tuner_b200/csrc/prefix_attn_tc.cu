@@ -19,8 +19,13 @@
 // any: scores by selection, and V by zeros written over the tile where some row may not see a key, since
 // 0 * V is not 0 for infinite or NaN V; what such a V gives to the rows that do see it is added at the end.
 //
-// Bound by the tensor pipe and the exponentials (16 a clock per SM: 256 x 128 of them take as long as the
-// tile's two MMAs at their nominal rate).
+// Bound by the chain of one half's tile, with the other half's beside it: S to P 2000 clocks (TMEM reads 300, maximum
+// 280, exponentials 1350 at 16 a clock per SM), P to the next S 1300 (PV 500, QK 560, the barriers' latency the rest).
+// The tensor pipe is active 0.51 of the time. Measured: 192 rows x 32 heads behind 65,536 keys (206 GFLOP) 194 us, 1.06
+// PFLOP/s, and 1.2 PFLOP/s without start and end, 0.7 of the measured bf16 rate; start and end are some 25 us (first
+// reads of offsets, pages, Q, K, the parts). Tried and slower: two threads a row (253 us), the product of the first 64
+// keys begun before the last exponentials (196), each TMEM read beside the maximum of the columns before (206), a
+// quarter of the exponentials as polynomials (213), S read twice in rolled loops for fewer registers (241).
 #include <type_traits>
 
 #include "attn_line.cuh"

@@ -14,7 +14,8 @@
 // SMs in one launch: each warp sums an equal piece of the row, the pieces' sums go to every CTA through
 // distributed shared memory, and the CTA whose warp holds the drawn index reads that piece again (from L2),
 // a few values a thread, to find it. What is left is latency: offsets, tokens, the tested numbers, the row, the
-// exchange and the piece are dependent reads (8 us for one sequence).
+// exchange and the piece are dependent reads. Measured: one sequence over 32064 fp32 values 6.0 us; 64 sequences of up to
+// 6 rows over 128256 values 17.6 us, of which the rows' 53 MB take 10; 155 over 49999 fp16 values 14.0 us.
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
