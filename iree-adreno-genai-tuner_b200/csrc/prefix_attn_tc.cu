@@ -23,7 +23,8 @@
 // 280, exponentials 1350 at 16 a clock per SM), P to the next S 1300 (PV 500, QK 560, the barriers' latency the rest).
 // The tensor pipe is active 0.51 of the time. Measured: 192 rows x 32 heads behind 65,536 keys (206 GFLOP) 194 us, 1.06
 // PFLOP/s, and 1.2 PFLOP/s without start and end, 0.7 of the measured bf16 rate; start and end are some 25 us (first
-// reads of offsets, pages, Q, K, the parts). Tried and slower: two threads a row (253 us), the product of the first 64
+// reads of offsets, pages, Q, K, the parts). Tried and slower: two threads a row (253 us), S in two buffers of 64 keys with
+// the next products begun two ahead (243: an MMA of 64 columns takes as long as one of 128), the product of the first 64
 // keys begun before the last exponentials (196), each TMEM read beside the maximum of the columns before (206), a
 // quarter of the exponentials as polynomials (213), S read twice in rolled loops for fewer registers (241).
 #include <type_traits>
