@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
 
   if (warp == 4 && count) {
     // producer: lane l brings box l of each tile; its page is looked up one tile ahead
-    const int box = min(a.kv.page_size, kMmKeys), boxes = kMmKeys / box;
+    const int box = page_box(a.kv.page_size, kMmKeys), boxes = kMmKeys / box;
     Cursor c = line.at(u0);
     auto page_of = [&]() {
       int page = -1;
@@ -1033,7 +1033,7 @@ int launch(const PrefixArgs& a, cudaStream_t st) {
     e = launch_wide<T, HD>(a, st);
   } else if constexpr (HD >= 64) {
     CUtensorMap tk, tv;
-    const int box = std::min(a.kv.page_size, kMmKeys);
+    const int box = page_box(a.kv.page_size, kMmKeys);
     if (int rc = make_tmap_pages(&tk, a.kv, a.kv.k, box)) return rc;
     if (int rc = make_tmap_pages(&tv, a.kv, a.kv.v, box)) return rc;
     e = a.mm_rows == 8 ? launch_narrow<T, HD, 8>(a, tk, tv, st) : launch_narrow<T, HD, 16>(a, tk, tv, st);

@@ -44,6 +44,13 @@ constexpr int kTcMaxBatch = 2048;  // the sequences' table shares the tensor-cor
 constexpr int kTcMinUnits = 500;
 constexpr int kTcMinRows = 64;     // rows x heads of a sequence from which it takes the own keys
 
+// Rows of a TMA box: the largest power of two that divides both the page (a multiple of 8) and the tile, so that no box
+// crosses a page or a tile.
+__host__ __device__ inline int page_box(int page_size, int tile) {
+  const int low = page_size & -page_size;
+  return low < tile ? low : tile;
+}
+
 // whether the kernels that load by TMA can read this cache
 bool prefix_tc_takes(const q4b_paged_kv& kv);
 int prefix_tc_run(const PrefixArgs& a, cudaStream_t st);

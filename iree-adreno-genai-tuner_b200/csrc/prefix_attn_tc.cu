@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == 8) {
       // producer: an item's run of n tiles is n + 1 entries of the ring, entry p its V tile p - 1 and K tile p: what one round of
       // the MMA thread needs, under one barrier
-      const int box = min(a.kv.page_size, kTcKeys), boxes = kTcKeys / box;
+      const int box = page_box(a.kv.page_size, kTcKeys), boxes = kTcKeys / box;
       int x = 0;
       bool ok = true;
       for (Segs g(line, run_own, run_prefix); ok && g.valid(); g.next()) {
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 template <typename T, int HD>
 int launch(const PrefixArgs& a, cudaStream_t st) {
   CUtensorMap tk, tv;
-  const int box = a.kv.page_size < kTcKeys ? a.kv.page_size : kTcKeys;
+  const int box = page_box(a.kv.page_size, kTcKeys);
   if (int rc = make_tmap_pages(&tk, a.kv, a.kv.k, box)) return rc;
   if (int rc = make_tmap_pages(&tv, a.kv, a.kv.v, box)) return rc;
   auto kern = prefix_tc_kernel<T, HD>;
@@ -634,13 +634,10 @@ int launch(const PrefixArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-// Pages that a 128-key tile holds whole, or that hold whole tiles, in boxes of full swizzle groups (8 rows);
-// strides that a tensor map can describe.
+// Pages of whole swizzle groups (8 rows), and strides that a tensor map can describe.
 bool prefix_tc_takes(const q4b_paged_kv& kv) {
-  const int ps = kv.page_size;
-  const bool boxes = ps % 8 == 0 && (ps % kTcKeys == 0 || kTcKeys % ps == 0);
   const bool strides = kv.slot_stride > 0 && (kv.n_kv_heads == 1 || kv.head_stride > 0) && (kv.n_pages == 1 || kv.page_stride > 0);
-  return kv.head_dim >= 64 && boxes && strides;
+  return kv.head_dim >= 64 && kv.page_size % 8 == 0 && strides;
 }
 
 int prefix_tc_run(const PrefixArgs& a, cudaStream_t st) {

@@ -161,6 +161,10 @@ ATTEND = [
     ([(1, 1)] * 129, 8, 3000, 16, 8, 64),
     ([(2, 40)] * 100, 256, 3500, 8, 8, 128),
     ([(1, 0)] * 40, 128, 12800, 8, 8, 64),  # no own keys; 40 rows; whole tiles
+    # pages that are no power of two
+    ([(1, 5)] * 150, 24, 4500, 8, 4, 64),
+    ([(70, 200), (1, 90), (9, 9)], 48, 333, 3, 1, 128),
+    ([(90, 700), (2, 2)], 192, 4000, 16, 4, 128),
     # many rows from pages that no TMA box fits
     ([(70, 200), (1, 90)], 20, 333, 3, 1, 128),
     ([(40, 100)] * 3, 1, 65, 4, 2, 64),
@@ -595,6 +599,57 @@ def test_step_in_graphs_and_streams(q4b):
         for x, y in zip(list(out) + [s["kp"], s["vp"]], ref):
             live = slice(0, 9) if x.shape[0] == 11 else slice(None)
             assert torch.equal(x[live], y[live])
+
+
+def test_attend_many_sequences_and_no_tables(q4b):
+    """The largest batch that the kernels take, and sequences without pages of their own."""
+    _run_attend(q4b, _attend_case([(1, 2), (0, 3), (1, 0), (2, 9)] * 1024, 8, 60, 2, 1, 64, torch.float16, 13), 8)
+    b, q, kp, vp = _attend_case([(1, 0), (2, 0)], 16, 40, 4, 2, 64, torch.float16, 3)
+    b["page_table"] = b["page_table"][:, :0]
+    _run_attend(q4b, (b, q, kp, vp), 16)
+
+
+def test_large_steps_on_two_streams(q4b):
+    """Steps that use the tensor cores, eager and replayed from graphs at once on two streams, with lengths that change."""
+    cases = [_attend_case([(1, 100)] * 60 + [(40, 300)], 16, 5000, 16, 4, 128, torch.float16, s) for s in (1, 2)]
+    devs = [_dev(c[0]) for c in cases]
+    call = lambda c, d: q4b.prefix_attention(c[1], c[2], c[3], d["prefix_pages"], 5000, d["page_table"], d["seq_lens"],  # noqa: E731
+                                             d["q_start"])
+    graphs, outs = [], []
+    for c, d in zip(cases, devs):
+        call(c, d)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(c, d))
+        graphs.append(g)
+    for d in devs:
+        d["seq_lens"].sub_(torch.arange(61, dtype=torch.int32, device=DEV))
+        d["q_start"].copy_(torch.cat([torch.arange(31, dtype=torch.int32), torch.full((30,), 30, dtype=torch.int32),
+                                      torch.tensor([70], dtype=torch.int32)]))
+    refs = []
+    for c, d in zip(cases, devs):
+        b = dict(c[0], seq_lens=d["seq_lens"].cpu().numpy(), q_start=d["q_start"].cpu().numpy())
+        refs.append(R.attention(_f64(c[1]), _f64(c[2]), _f64(c[3]), b, 16))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    eager = [[], []]
+    for n in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                if n % 2:
+                    eager[i].append(call(cases[i], devs[i]))
+                else:
+                    graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        live = ~np.isnan(refs[i]).any(axis=(1, 2))
+        assert live[:70].all() and not live[70:].any()
+        for o in eager[i] + [outs[i]]:
+            got = _f64(o).reshape(refs[i].shape)
+            _check_attend(np.where(live[:, None, None], got, 0), np.where(live[:, None, None], refs[i], 0), _f64(cases[i][3]),
+                          torch.float16, live)
+    assert q4b.lib().q4b_device_status(1) == 0
 
 
 def test_results_do_not_depend_on_timing(q4b):
