@@ -961,17 +961,35 @@ Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv, bool wide
   if (prefix_here) p.mm.prefix_units = prefix_units(rows, g, Hkv, b.prefix_len, p.mm_rows, kMmKeys);
   int mm_sms = kSms;
   // Small steps, where either kernel's start and end (some 10 us of launch, first reads and last parts) weigh as much as
-  // its tiles: both at once, the SMs shared by the measured time of their tiles and a guess at the own keys (0.6 of what
-  // the page tables hold), instead of one behind the other. 61 sequences of 5 drafts behind 4099 keys: 45 us against 52;
-  // 192 single tokens behind 16384 keys, where a wrong guess costs more than the start: 207 at best against 210.
+  // its tiles: both at once, on disjoint SMs, instead of one behind the other. 61 sequences of 5 drafts behind 4099 keys: 45
+  // us against 52; 192 single tokens behind 16384 keys, where a wrong guess at the own keys (0.6 of what the page tables
+  // hold) costs more than the start: 207 at best against 210.
   const int per_sequence = (R + std::max(b.batch, 1) - 1) / std::max(b.batch, 1);
   if (tc_prefix && per_sequence <= kTcMinRows && p.mm_rows < 64) {
-    const double tc_us = p.tc.prefix_units / (double)kSms * (kv.head_dim == 128 ? 2.0 : 1.4);
-    const double mm_us = (double)b.batch * Hkv * ((per_sequence + p.mm_rows - 1) / p.mm_rows) *
-                         (0.6 * b.table_width * kv.page_size / kMmKeys) / (mm_ctas_per_sm(kv.head_dim) * kSms) * 1.3;
+    const int items = Hkv * ((R + kTcRows - 1) / kTcRows), tiles = (b.prefix_len + kTcKeys - 1) / kTcKeys;
+    const double tile_us = kv.head_dim == 128 ? 2.0 : 1.6;
+    // row tiles of a sequence (ragged: a little above the mean), an item's start and end as 1.3 tiles
+    const double row_tiles = rows <= b.batch ? (per_sequence + p.mm_rows - 1) / p.mm_rows
+                                             : std::max(1.0, (double)R / std::max(b.batch, 1) / p.mm_rows + 0.2);
+    const double mm_us = b.batch * (double)Hkv * row_tiles * (0.6 * b.table_width * kv.page_size / kMmKeys + 1.3) * 1.3 /
+                         (mm_ctas_per_sm(kv.head_dim) * kSms);
+    const double tc_us = (double)items * tiles * tile_us / kSms;
     if (tc_us + mm_us < 40) {
-      p.tc_ctas = std::min(std::max((int)(kSms * tc_us / (tc_us + mm_us)), kSms / 6), kSms * 3 / 4);
-      mm_sms = kSms - p.tc_ctas;
+      // SMs for the prefix: a multiple of its items, so that no CTA has parts of two (that costs some 3 us), or the share of
+      // the tiles' time. More CTAs an item are more parts for the join, 0.5 us each. Measured against the share alone: 24
+      // sequences of 6 behind 3000 keys 35 us and 49, 32 single tokens behind 2048 25 and 28.5, 64 behind 1500 42.5 and 40.
+      auto cost = [&](int ctas, double each, double parts) {
+        return std::max(2.0 + each * tile_us, mm_us * kSms / (kSms - ctas)) + 0.5 * parts;
+      };
+      int best = 0;
+      double least = 1e30;
+      auto take = [&](int ctas, double us) {
+        if (us < least) least = us, best = ctas;
+      };
+      for (int c = kSms / 6; c <= kSms * 3 / 4; c += 4) take(c, cost(c, items * (double)tiles / c + 3.0 / tile_us, 1.0 + c / (double)items));
+      for (int m = 1; m <= tiles && m * items <= kSms * 3 / 4; ++m) take(m * items, cost(m * items, (tiles + m - 1) / m, m));
+      p.tc_ctas = best;
+      mm_sms = kSms - best;
     }
   }
   p.mm_ctas = mm_ctas_per_sm(kv.head_dim) * mm_sms;
