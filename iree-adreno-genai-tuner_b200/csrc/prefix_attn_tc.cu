@@ -26,7 +26,11 @@
 // reads of offsets, pages, Q, K, the parts). Tried and slower: two threads a row (253 us), S in two buffers of 64 keys with
 // the next products begun two ahead (243: an MMA of 64 columns takes as long as one of 128), the product of the first 64
 // keys begun before the last exponentials (196), each TMEM read beside the maximum of the columns before (206), a
-// quarter of the exponentials as polynomials (213), S read twice in rolled loops for fewer registers (241).
+// quarter of the exponentials as polynomials (213), S read twice in rolled loops for fewer registers (241), weights against
+// the old maximum and once more if it was outgrown (203), a ring of 5 single tiles (200), with head_dim 64 columns of their
+// own for P and the next S begun when the last has been read (180 against 162). Neither pipe is full (tensor 0.50,
+// exponentials 0.56, issue 0.33): a warp alone on its scheduler waits 2.3 clocks an instruction for its last results, and
+// more warps have no registers.
 #include <type_traits>
 
 #include "attn_line.cuh"

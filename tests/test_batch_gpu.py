@@ -161,6 +161,8 @@ ATTEND = [
     ([(1, 1)] * 129, 8, 3000, 16, 8, 64),
     ([(2, 40)] * 100, 256, 3500, 8, 8, 128),
     ([(1, 0)] * 40, 128, 12800, 8, 8, 64),  # no own keys; 40 rows; whole tiles
+    # a prefix so long that the kernels take turns, its items on a multiple of them of CTAs
+    ([(1, 5), (1, 300), (1, 0)], 128, 126_500, 6, 3, 128),
     # pages that are no power of two
     ([(1, 5)] * 150, 24, 4500, 8, 4, 64),
     ([(70, 200), (1, 90), (9, 9)], 48, 333, 3, 1, 128),
