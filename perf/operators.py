@@ -22,12 +22,10 @@ KEPT = 0.7
 _TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
 
 
-_PACKAGE = str(pathlib.Path(__file__).resolve().parents[1] / "iree-adreno-genai-tuner_b200")
-
-
 def _q4b():
-    if _PACKAGE not in sys.path:
-        sys.path.insert(0, _PACKAGE)
+    pkg = str(pathlib.Path(__file__).resolve().parents[1] / "iree-adreno-genai-tuner_b200")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
     import q4b
     return q4b
 
