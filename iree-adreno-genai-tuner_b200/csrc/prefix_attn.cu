@@ -65,6 +65,10 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Zeros over shared memory that ldsm4 reads: a volatile asm like those, so that the compiler keeps their order.
+__device__ __forceinline__ void st_zero16(uint32_t dst) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -737,7 +741,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
             const int key = k0 + x / C::CHUNKS;
             uint4* v = reinterpret_cast<uint4*>(smem + (vs - s0) + sw_tma(key, x % C::CHUNKS));
             if (key0 + key >= cur.limit) {
-              *v = make_uint4(0, 0, 0, 0);
+              st_zero16(smem_u32(v));
             } else if (key0 + key >= cur.first) {
               const uint4 old = *v;
               const uint32_t vv[4] = {old.x, old.y, old.z, old.w};
@@ -747,6 +751,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
           }
           odd = __any_sync(0xffffffffu, found);
           wrote = true;
+          __syncwarp();  // the zeros of other lanes: a vote does not order memory
         }
         const bool whole = mask == ~0ull && key0 + kMmKeys <= cur.first;
         w.tile(ks, vs, k0, key0, mask, whole, odd, a.scale2, lane);

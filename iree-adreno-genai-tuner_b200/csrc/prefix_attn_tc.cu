@@ -476,6 +476,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
           fence_async_smem();
+          __syncwarp();  // the loops above end lane by lane, the TMEM loads below want the warp together
         }
         tc_fence_after();
         uint32_t sc[4][32];
@@ -564,6 +565,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
+          __syncwarp();  // behind the loop over `odd` keys, whose length differs by lane
           if (n > 0) {
             tmem_ld_async(to + 32 * c, o);
             tmem_ld_wait(o);
