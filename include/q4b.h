@@ -250,6 +250,11 @@ int q4b_prefix_attention(const void* q, long long q_stride, long long q_head_str
                          float scale, const int32_t* prefix_pages, const q4b_batch* batch, const q4b_paged_kv* kv,
                          void* out, void* workspace, size_t workspace_bytes, q4b_stream_t stream);
 
+/* The longest that a wait in the attention kernels of calls from now on may take, in ns (1e9 unless set; captured graphs keep
+ * theirs). Rows whose work gave up are NaN, and q4b_device_status reports Q4B_ETIMEOUT. With 0 every wait gives
+ * up, which shows a caller's handling of that report without a fault. */
+void q4b_prefix_attention_wait_limit(unsigned long long ns);
+
 /* Verification of drafted tokens (the greedy head of llama_q4.py:237-239, for sampling with a draft model).
  * tokens [rows]: the step's input tokens; row q_start[b] is b's last sure token and the rows behind it
  * its drafts. Row r of target [rows, vocab] (and of draft, the distributions the drafts were drawn from; NULL:

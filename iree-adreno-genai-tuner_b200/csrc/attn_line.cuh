@@ -7,6 +7,11 @@
 
 namespace q4b {
 
+// A wait within the call's limit; a limit of zero gives up without a look.
+__device__ __forceinline__ bool wait_for(const PrefixArgs& a, uint64_t* bar, uint32_t parity) {
+  return a.wait_ns && mbar_wait_bounded(bar, parity, a.wait_ns);
+}
+
 // First unit of CTA c, and the CTA that holds unit u, for `units` units over `ctas` CTAs.
 __device__ __forceinline__ int cta_first(int c, int units, int ctas) { return (int)((long long)c * units / ctas); }
 // The largest c with cta_first(c) <= u, i.e. with c * units <= (u + 1) * ctas - 1: by a guess in fp32 (off by one at most:

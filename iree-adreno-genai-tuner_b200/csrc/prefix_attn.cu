@@ -42,6 +42,8 @@ constexpr int kMaxBatch = 4096;
 
 __device__ unsigned g_narrow_status = 0;
 
+std::atomic<unsigned long long> g_wait_ns{kWaitLimitNs};
+
 template <int HD>
 struct Cfg {
   static constexpr int STAGES = HD == 128 ? 3 : 4;
@@ -631,7 +633,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
   uint8_t* smem = smem_raw + (s0 - smem_u32(smem_raw));
   __shared__ uint64_t full[C::STAGES], empty[C::STAGES];
   __shared__ unsigned long long s_mask[C::STAGES];
-  __shared__ int s_scan[kNarrowThreads / 32], s_fail;
+  __shared__ int s_scan[kNarrowThreads / 32], s_fail, s_issued;
   __shared__ float s_m[4][TR], s_l[4][TR];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 4);
     }
-    s_fail = 0;
+    s_fail = s_issued = 0;
     fence_mbar_init();
     tma_prefetch_map(&tk);
     tma_prefetch_map(&tv);
@@ -674,7 +676,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
         page = __ldg((c.b < 0 ? a.prefix_pages : a.b.page_table + c.b * a.b.table_stride) + key / a.kv.page_size);
       return page;
     };
-    int page = page_of(), issued = 0;
+    int page = page_of();
     for (int i = 0; i < count; ++i) {
       const int s = i % C::STAGES, key = c.tile * kMmKeys + lane * box, left = c.limit - key, h = c.h;
       const bool there = page >= 0 && page < a.kv.n_pages;  // lanes without a box or with no key left: not
@@ -684,11 +686,15 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
       unsigned lo = __reduce_or_sync(0xffffffffu, (unsigned)mask), hi = __reduce_or_sync(0xffffffffu, (unsigned)(mask >> 32));
       bool ok = true;
       if (lane == 0) {
-        ok = i < C::STAGES || mbar_wait_bounded(&empty[s], (i / C::STAGES - 1) & 1, kWaitLimitNs);
-        if (ok) {
+        ok = i < C::STAGES || wait_for(a, &empty[s], (i / C::STAGES - 1) & 1);
+        // A warp that gave up no longer waits for full, so its arrivals do not mean that the slot's copies have landed: nothing
+        // more is brought then (a second arrival on a phase whose copies are in flight would be undefined).
+        if (ok && !*fail) {
           s_mask[s] = (unsigned long long)hi << 32 | lo;
           mbar_arrive_expect_tx(&full[s], C::STAGE);
+          s_issued = i + 1;
         } else {
+          ok = false;
           *fail = 1;
         }
       }
@@ -702,14 +708,11 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
           tma_load_4d(dst + C::HALF + x * kMmKeys * 128, &tv, 64 * x, slot, h, from, &full[s]);
         }
       }
-      issued = i + 1;
-      if (issued < count) {
+      if (i + 1 < count) {
         line.next(c);
         page = page_of();
       }
     }
-    if (lane == 0 && *fail)  // leave no copy in flight
-      for (int i = max(issued - C::STAGES, 0); i < issued; ++i) mbar_wait_bounded(&full[i % C::STAGES], (i / C::STAGES) & 1, kWaitLimitNs);
   } else if (warp < 4 && count) {
     Cursor cur = line.at(u0);
     Narrow<T, HD, TR> w;
@@ -724,7 +727,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
       }
       const int s = i % C::STAGES, key0 = cur.tile * kMmKeys;
       // After a wait that gave up, the run goes on without waiting (the warps meet at barriers), to no use.
-      if (!*fail && !mbar_wait_bounded(&full[s], (i / C::STAGES) & 1, kWaitLimitNs)) *fail = 1;
+      if (!*fail && !wait_for(a, &full[s], (i / C::STAGES) & 1)) *fail = 1;
       __syncwarp();
       const uint32_t ks = s0 + s * C::STAGE, vs = ks + C::HALF;
       const unsigned long long mask = s_mask[s];
@@ -815,7 +818,11 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0 && *fail) atomicOr(&g_narrow_status, kStatusTimeout);
+  if (threadIdx.x == 0 && *fail) {
+    atomicOr(&g_narrow_status, kStatusTimeout);
+    for (int i = max(s_issued - C::STAGES, 0); i < s_issued; ++i)  // leave no copy in flight
+      mbar_wait_bounded(&full[i % C::STAGES], (i / C::STAGES) & 1, kWaitLimitNs);
+  }
   join_records<TR, kNarrowThreads>(a, table, bad, units, s_scan);
 }
 
@@ -1145,6 +1152,7 @@ extern "C" int q4b_prefix_attention(const void* q, long long q_stride, long long
   a.mm_o = reinterpret_cast<float*>(base + w.mm_o);
   a.tc_ml = reinterpret_cast<float2*>(base + w.tc_ml);
   a.tc_o = reinterpret_cast<float*>(base + w.tc_o);
+  a.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
   const cudaStream_t st = as_stream(stream);
   if (a.tc_ctas)
     if (int rc = prefix_tc_run(a, st)) return rc;
@@ -1155,3 +1163,5 @@ extern "C" int q4b_prefix_attention(const void* q, long long q_stride, long long
     default: return h16 ? launch<__half, 32>(a, st) : launch<__nv_bfloat16, 32>(a, st);
   }
 }
+
+extern "C" void q4b_prefix_attention_wait_limit(unsigned long long ns) { g_wait_ns.store(ns, std::memory_order_relaxed); }

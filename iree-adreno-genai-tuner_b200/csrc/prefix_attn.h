@@ -25,7 +25,7 @@ struct PrefixArgs {
   int mm_ctas;       // CTAs of the mma.sync kernel
   int mm_rows;       // its rows per row tile: 8 or 16 (narrow), 64 (wide)
   AttnLine tc, mm;
-  int4* rec;         // [rows]: where the join finds a row's own item (see RowRec)
+  int4* rec;         // [rows]: where the join finds a row's own item (join_records)
   int* totals;       // units of the mm line, own units of the tc line
   float2* row_ml;    // [2][rows * H] (max, sum) of items that one CTA did whole, prefix then own keys
   float* row_o;      // [2][rows * H][hd] their weighted V
@@ -33,6 +33,7 @@ struct PrefixArgs {
   float* mm_o;
   float2* tc_ml;     // [prefix, own][CTAs][2][kTcRows]
   float* tc_o;
+  unsigned long long wait_ns;  // limit of the kernels' waits
 };
 
 constexpr int kTcRows = 256, kTcKeys = 128, kTcCtas = 148;

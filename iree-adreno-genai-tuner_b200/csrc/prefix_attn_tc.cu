@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int p = 0; p <= n; ++p, ++x) {
           const int slot = x % C::SLOTS, r = x / C::SLOTS, j = s.t0 + p;
           if (lane == 0) {
-            ok = r == 0 || mbar_wait_bounded(&empty[slot], (r - 1) & 1, kWaitLimitNs);
+            ok = r == 0 || wait_for(a, &empty[slot], (r - 1) & 1);
             if (ok) {
               mbar_arrive_expect_tx(&full[slot], p == 0 || p == n ? C::TILE : 2 * C::TILE);
               s_issued = x + 1;
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // were most of this thread's time, and this thread was what the kernel waited for.
         const uint64_t q_desc = sw128_desc(base, 16, 1024), k_desc = sw128_desc(base + 2 * C::TILE, 16, 1024),
                        v_desc = sw128_desc(base + 3 * C::TILE, C::ATOM, 1024);
-        auto wait_full = [&](int x) { return mbar_wait_bounded(&full[x % C::SLOTS], (x / C::SLOTS) & 1, kWaitLimitNs); };
+        auto wait_full = [&](int x) { return wait_for(a, &full[x % C::SLOTS], (x / C::SLOTS) & 1); };
         auto qk = [&](int i, int x) {
           const uint64_t q = q_desc + i * (C::TILE >> 4), k = k_desc + x % C::SLOTS * (2 * C::TILE >> 4);
 #pragma unroll
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (n == 0) continue;
           ok = wait_full(x);
           for (int i = 0; ok && i < active; ++i) {
-            ok = mbar_wait_bounded(&q_full[i], (i ? items1 : items) & 1, kWaitLimitNs);
+            ok = wait_for(a, &q_full[i], (i ? items1 : items) & 1);
             if (!ok) break;
             tc_fence_after();
             qk(i, x);
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ++x;
             ok = wait_full(x);
             for (int i = 0; ok && i < active; ++i) {
-              ok = mbar_wait_bounded(&p_full[i], ((i ? tiles1 : tiles) + j) & 1, kWaitLimitNs);
+              ok = wait_for(a, &p_full[i], ((i ? tiles1 : tiles) + j) & 1);
               if (!ok) break;
               tc_fence_after();
               pv(i, x, j == 0);
@@ -376,11 +376,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tiles += n, ++items;
           if (active == 2) tiles1 += n, ++items1;
         }
-        if (!ok) {  // let what was issued end before the TMEM goes back
-          *fail = 1;
-          tc_commit(&drained);
-          mbar_wait_bounded(&drained, 0, kWaitLimitNs);
-        }
+        if (!ok) *fail = 1;
       }
       __syncwarp();
     }
@@ -435,7 +431,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (key0 + 4 * lane < s.c.limit) page = __ldg(pages + (key0 + 4 * lane) / a.kv.page_size);
         const unsigned there = __ballot_sync(0xffffffffu, page >= 0 && page < a.kv.n_pages);
         const bool edge = key0 + kTcKeys > s.c.first;  // some row does not see all of the tile's keys
-        ok = mbar_wait_bounded(&s_full[i], (tiles + j) & 1, kWaitLimitNs);
+        ok = wait_for(a, &s_full[i], (tiles + j) & 1);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -444,7 +440,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // Behind the wait for S: a half that sat out items may be ahead of the ring by more than the one phase that a
           // barrier's parity tells apart, but this tile's K is there, so its V is the barrier's current phase.
           const int xv = x + j + 1;
-          ok = mbar_wait_bounded(&full[xv % C::SLOTS], (xv / C::SLOTS) & 1, kWaitLimitNs);
+          ok = wait_for(a, &full[xv % C::SLOTS], (xv / C::SLOTS) & 1);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -549,7 +545,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (ok && g.valid()) load_q(g.s);  // the item's products with Q have ended
       if (ok && n > 0) {
-        ok = mbar_wait_bounded(&o_full[i], items & 1, kWaitLimitNs);
+        ok = wait_for(a, &o_full[i], items & 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
@@ -604,6 +600,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
+    if (*fail) {  // whoever gave up: let the products that were issued end before the TMEM goes back
+      if (lane == 0) {
+        tc_commit(&drained);
+        mbar_wait_bounded(&drained, 0, kWaitLimitNs);
+      }
+      __syncwarp();
+    }
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

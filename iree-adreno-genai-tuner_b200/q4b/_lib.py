@@ -120,6 +120,7 @@ SIGNATURES = {
     "q4b_prefix_attention": (c_int, [c_void_p, c_longlong, c_longlong, c_int, c_int, c_float, c_void_p,
                                      ctypes.POINTER(Batch), ctypes.POINTER(PagedKV), c_void_p, c_void_p, c_size_t,
                                      c_void_p]),
+    "q4b_prefix_attention_wait_limit": (None, [ctypes.c_ulonglong]),
     "q4b_verify_drafts": (c_int, [c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_int, c_void_p, c_void_p, c_int,
                                   c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "q4b_tp_init": (c_int, [c_int, c_int, c_void_p, c_int, ctypes.POINTER(c_void_p)]),

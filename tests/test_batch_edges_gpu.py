@@ -23,3 +23,33 @@ def test_rest_of_a_page_never_shows(q4b, hd, new, g, page):  # noqa: F811
     case = _attend_case(lens, page, 0, 2 * g, 2, hd, torch.float16, seed=page + g)
     out, _, live = _run_attend(q4b, case, page)
     assert live.all() and bool(torch.isfinite(out).all())
+
+
+# ---- prefix_attention: waits that give up ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens,prefix,H,Hkv,hd", [
+    ([(1, 700), (1, 90), (2, 33)] * 9, 0, 8, 2, 128),  # the narrow kernel
+    ([(1, 5)] * 150, 4500, 8, 4, 64),  # both, a few tiles each
+    ([(1, 1900)] * 40 + [(90, 2000)], 9000, 8, 2, 128),  # both, rings that go round, own keys on the tensor cores too
+])
+def test_waits_that_give_up_are_reported(q4b, lens, prefix, H, Hkv, hd):  # noqa: F811
+    """With a limit of zero every wait gives up: each row that has keys is NaN, none is stale, the status tells, and the next
+    call is right again. The waits end by themselves; nothing is left out or broken for it."""
+    L = q4b.lib()
+    case = _attend_case(lens, 16, prefix, H, Hkv, hd, torch.float16, seed=3)
+    b, q, kp, vp = case
+    d = _dev(b)
+    call = lambda: q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"])  # noqa: E731
+    assert L.q4b_device_status(1) == 0
+    L.q4b_prefix_attention_wait_limit(0)
+    try:
+        outs = [call() for _ in range(3)]
+        torch.cuda.synchronize()
+    finally:
+        L.q4b_prefix_attention_wait_limit(10**9)
+    for o in outs:
+        assert bool(torch.isnan(o).all())
+    assert L.q4b_device_status(1) == -3 and L.q4b_device_status(1) == 0
+    _run_attend(q4b, case, 16)
+    assert L.q4b_device_status(1) == 0
