@@ -202,8 +202,8 @@ int q4b_argmax(const float* logits, int n, int32_t* index, q4b_stream_t stream);
  * page_table[b, s / page_size], at position prefix_len + s. The prefix_len keys in front are shared by all
  * sequences (0: none). Device arrays, read when the work runs, so a captured graph follows them; rows
  * behind q_start[batch] are left as they were. Values are bounded on the device: q_start (which must
- * not decrease) is clamped to [0, rows], seq_lens to the table's keys, and a page id outside [0, n_pages)
- * holds no keys (appends to it are dropped, attention does not see them). */
+ * not decrease) is clamped to [0, rows]; keys behind the table's table_width pages, and those of a page id outside
+ * [0, n_pages), are not there (appends to them are dropped, attention does not see them). */
 typedef struct q4b_batch {
   const int32_t* q_start;    /* [batch + 1] */
   const int32_t* seq_lens;   /* [batch] */

@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
     if (b >= 0) {
       const int2 r = batch_rows(a.b.q_start, b, a.rows);
       const long long cap = (long long)a.b.table_width * a.kv.page_size;
-      const long long len = min((long long)max(__ldg(a.b.seq_lens + b), 0), cap);
-      const long long s = len - (r.y - r.x) + (t - r.x);
+      // by the length as it is: behind the table's keys there is no slot, and no other token's slot is written instead
+      const long long s = (long long)__ldg(a.b.seq_lens + b) - (r.y - r.x) + (t - r.x);
       pos = a.b.prefix_len + s;
       state = a.rot == 0 || (pos >= 0 && pos < a.table_rows) ? kLive : kZero;
       if (state == kLive && s >= 0 && s < cap) {

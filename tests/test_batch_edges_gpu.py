@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import batch_ref as R
-from test_batch_gpu import DEV, _attend_case, _dev, _f64, _run_attend, q4b  # noqa: F401
+from test_batch_gpu import DEV, _attend_case, _dev, _f64, _run_append, _run_attend, q4b  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,29 @@ def test_waits_that_give_up_are_reported(q4b, lens, prefix, H, Hkv, hd):  # noqa
     assert L.q4b_device_status(1) == -3 and L.q4b_device_status(1) == 0
     _run_attend(q4b, case, 16)
     assert L.q4b_device_status(1) == 0
+
+
+# ---- paged_rope_append: sequences that outgrow their tables ---------------------------------------------
+
+
+@pytest.mark.parametrize("lens,width", [
+    ([(1, 33), (1, 32), (2, 20)], 4),  # one token behind the last slot; the last slot; inside
+    ([(4, 34), (3, 50), (40, 45)], 4),  # rows on both sides of the table's end, all behind it, a chunk across it
+    ([(2, 2), (1, 9)], 0),  # no pages at all
+    ([(3, -5), (2, 1), (1, 0)], 4),  # negative, and shorter than the new rows
+])
+@pytest.mark.parametrize("prefix", [0, 7])
+def test_append_behind_the_table_is_dropped(q4b, lens, width, prefix):  # noqa: F811
+    """A row keeps its position whatever the table holds: it is rotated there, and written nowhere else."""
+    page, H, Hkv, hd = 8, 4, 2, 64
+    rng = np.random.default_rng(len(lens) + width)
+    b = dict(q_start=np.concatenate([[0], np.cumsum([n for n, _ in lens])]).astype(np.int32), prefix_len=prefix,
+             seq_lens=np.array([o for _, o in lens], dtype=np.int32),
+             page_table=rng.permutation(20)[:len(lens) * width].reshape(len(lens), width).astype(np.int32),
+             prefix_pages=np.zeros(0, dtype=np.int32), rows=sum(n for n, _ in lens))
+    g = torch.Generator(device=DEV).manual_seed(width)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
+    q, k, v = rn(b["rows"], H, hd), rn(b["rows"], Hkv, hd), rn(b["rows"], Hkv, hd)
+    kp, vp = (rn(20, page, Hkv, hd).half() for _ in range(2))
+    ang = torch.arange(100, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(hd // 2, dtype=torch.float64) / (hd // 2))
+    _run_append(q4b, (b, q, k, v, kp, vp, ang.cos().float().to(DEV), ang.sin().float().to(DEV)), "half", page, "float16")
