@@ -28,12 +28,15 @@ __device__ __forceinline__ int cta_of(int u, int units, int ctas) {
 struct BatchTable {
   int* cum;  // [batch + 1] units of this line in front of sequence b, behind the prefix's
   int* q0;   // [batch + 1] first row
-  int* len;  // [batch] own keys
+  int* len;  // [batch] own keys, those behind the page table among them
 };
+
+// Own keys of a sequence that its page table holds
+__device__ __forceinline__ int held(const PrefixArgs& a, int len) { return min(len, a.table_keys); }
 
 __device__ __forceinline__ int line_units(const PrefixArgs& a, const AttnLine& line, int n, int len, int tr, int tk) {
   const int r = n * a.g;
-  return r > line.own_lo && r <= line.own_hi ? a.Hkv * ((r + tr - 1) / tr) * ((len + tk - 1) / tk) : 0;
+  return r > line.own_lo && r <= line.own_hi ? a.Hkv * ((r + tr - 1) / tr) * ((held(a, len) + tk - 1) / tk) : 0;
 }
 
 // Exclusive running sum of `mine` over the block's threads, and the total; `s` holds a word per warp and one more.
@@ -64,14 +67,13 @@ __device__ __forceinline__ int block_scan(int mine, int* s, int& total) {
 template <int THREADS>
 __device__ __forceinline__ bool batch_table(const PrefixArgs& a, const BatchTable& s) {
   const int B = a.b.batch;
-  const long long cap = min((long long)a.b.table_width * a.kv.page_size, 0x7fffffffll - kTcKeys);
   bool bad = false;
   for (int b = threadIdx.x; b <= B; b += THREADS) {
     const int q = __ldg(a.b.q_start + b);
     s.q0[b] = min(max(q, 0), a.rows);
     if (b < B) {
       bad |= __ldg(a.b.q_start + b + 1) < q;
-      s.len[b] = (int)min((long long)max(__ldg(a.b.seq_lens + b), 0), cap);
+      s.len[b] = min(max(__ldg(a.b.seq_lens + b), 0), 0x7fffffff - kTcRows);  // row_limit counts on from here
     }
   }
   return __syncthreads_or(bad);
@@ -100,7 +102,7 @@ struct Cursor {
   int b;      // sequence, -1: the prefix
   int h, rt;  // KV head, row tile
   int tile, tiles, row_tiles;
-  int q0, n, len;  // first row, rows and keys of the sequence (prefix: 0, all rows, prefix_len)
+  int q0, n, len;  // first row, rows and keys (that are held) of the sequence (prefix: 0, all rows, prefix_len)
   int nrows;       // rows of this row tile
   int limit;       // keys that its last row sees
   int first;       // keys that its first row sees
@@ -118,8 +120,9 @@ struct Line {
       c.limit = c.first = c.len;
     } else {
       const int j0 = c.rt * TR / a.g, j1 = (c.rt * TR + c.nrows - 1) / a.g;
-      c.first = min(max(c.len - c.n + j0 + 1, 0), c.len);
-      c.limit = min(max(c.len - c.n + j1 + 1, 0), c.len);
+      const int seen = s.len[c.b] - c.n;  // own keys in front of the first row; negative: fewer keys than rows
+      c.first = min(max(seen + j0 + 1, 0), c.len);
+      c.limit = min(max(seen + j1 + 1, 0), c.len);
     }
   }
   __device__ __forceinline__ void sequence(Cursor& c) const {
@@ -130,7 +133,7 @@ struct Line {
     } else {
       c.q0 = s.q0[c.b];
       c.n = s.q0[c.b + 1] - c.q0;
-      c.len = s.len[c.b];
+      c.len = held(a, s.len[c.b]);
     }
     c.row_tiles = (c.n * a.g + TR - 1) / TR;
     c.tiles = (c.len + TK - 1) / TK;
@@ -179,8 +182,8 @@ struct Line {
 };
 
 // keys that row r of the cursor's row tile sees
-__device__ __forceinline__ int row_limit(const PrefixArgs& a, const Cursor& c, int r, int tr) {
-  return c.b < 0 ? c.len : min(c.len - c.n + (c.rt * tr + r) / a.g + 1, c.len);
+__device__ __forceinline__ int row_limit(const PrefixArgs& a, const BatchTable& s, const Cursor& c, int r, int tr) {
+  return c.b < 0 ? c.len : min(s.len[c.b] - c.n + (c.rt * tr + r) / a.g + 1, c.len);
 }
 
 // Where a run of an item puts (max, sum) and weighted V of row r of its row tile: by the output row if the run is the

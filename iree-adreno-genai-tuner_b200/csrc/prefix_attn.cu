@@ -125,7 +125,7 @@ struct Wide {
   float m[2], l[2];
   int lim[2];  // keys that this lane's two rows see
 
-  __device__ __forceinline__ void start(const PrefixArgs& a, const Cursor& c, int r0, int lane) {
+  __device__ __forceinline__ void start(const PrefixArgs& a, const BatchTable& s, const Cursor& c, int r0, int lane) {
     const T* qp[2];
     bool on[2];
 #pragma unroll
@@ -133,7 +133,7 @@ struct Wide {
       const int r = r0 + (lane >> 2) + 8 * i;
       on[i] = r < c.nrows;
       qp[i] = q_row<T>(a, c, 64, r) + 2 * (lane & 3);
-      lim[i] = row_limit(a, c, r, 64);
+      lim[i] = row_limit(a, s, c, r, 64);
       m[i] = -INFINITY;
       l[i] = 0.0f;
     }
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_wide_kernel(Pr
   bool split_keys = false;  // the warps share the tile's keys, not the rows
   auto start = [&]() {
     split_keys = cur.nrows <= 16;
-    w.start(a, cur, split_keys ? 0 : warp * 16, lane);
+    w.start(a, table, cur, split_keys ? 0 : warp * 16, lane);
   };
   if (count) start();
   bool began = cur.tile == 0;  // the item's first unit is this CTA's
@@ -498,7 +498,7 @@ struct Narrow {
     if (r < min(TR, c.nrows))
       asm volatile("prefetch.global.L1 [%0];" ::"l"(q_row<T>(a, c, TR, r) + lane % LINES * 64));
   }
-  __device__ __forceinline__ void start(const PrefixArgs& a, const Cursor& c, int lane) {
+  __device__ __forceinline__ void start(const PrefixArgs& a, const BatchTable& s, const Cursor& c, int lane) {
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const int r = 8 * n + (lane >> 2);
@@ -513,7 +513,7 @@ struct Narrow {
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        lim[n][e] = row_limit(a, c, 8 * n + 2 * (lane & 3) + e, TR);
+        lim[n][e] = row_limit(a, s, c, 8 * n + 2 * (lane & 3) + e, TR);
         m[n][e] = -INFINITY;
         l[n][e] = 0.0f;
       }
@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
   } else if (warp < 4 && count) {
     Cursor cur = line.at(u0);
     Narrow<T, HD, TR> w;
-    w.start(a, cur, lane);
+    w.start(a, table, cur, lane);
     bool began = cur.tile == 0;  // the item's first unit is this CTA's
     for (int i = 0; i < count; ++i) {
       const bool ends = cur.tile == cur.tiles - 1, run_ends = ends || i + 1 == count;
@@ -813,7 +813,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
         if (lane == 0) mbar_arrive(&empty[s]);
         cur = next;
         began = true;
-        w.start(a, cur, lane);
+        w.start(a, table, cur, lane);
       }
     }
   }
@@ -1142,6 +1142,7 @@ extern "C" int q4b_prefix_attention(const void* q, long long q_stride, long long
   a.rows = rows, a.H = n_heads, a.Hkv = kv->n_kv_heads, a.g = n_heads / kv->n_kv_heads;
   a.scale2 = scale * 1.44269504088896340736f;
   a.b = *batch, a.kv = *kv, a.prefix_pages = prefix_pages, a.out = out;
+  a.table_keys = (int)std::min((long long)batch->table_width * kv->page_size, 0x7fffffffll - kTcKeys);
   a.tc_ctas = p.tc_ctas, a.mm_ctas = p.mm_ctas, a.mm_rows = p.mm_rows, a.tc = p.tc, a.mm = p.mm;
   char* base = static_cast<char*>(workspace);
   a.rec = reinterpret_cast<int4*>(base + w.rec);

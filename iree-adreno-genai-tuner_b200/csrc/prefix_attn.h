@@ -18,6 +18,7 @@ struct PrefixArgs {
   int rows, H, Hkv, g;  // g = H / Hkv
   float scale2;         // scale * log2(e)
   q4b_batch b;
+  int table_keys;  // keys that a row of the page table holds
   q4b_paged_kv kv;
   const int32_t* prefix_pages;
   void* out;  // [rows, H * hd]

@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (g.valid()) load_q(g.s);
         continue;
       }
-      const int lim = row_limit(a, s.c, i * kHalf + row, kTcRows);
+      const int lim = row_limit(a, table, s.c, i * kHalf + row, kTcRows);
       const int32_t* pages = page_row(a, s.c);
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; ok && j < n; ++j) {

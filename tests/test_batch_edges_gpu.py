@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import batch_ref as R
-from test_batch_gpu import DEV, _attend_case, _dev, _f64, _run_append, _run_attend, q4b  # noqa: F401
+from test_batch_gpu import DEV, _attend_case, _check_attend, _dev, _f64, _run_append, _run_attend, q4b  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,36 @@ def test_append_behind_the_table_is_dropped(q4b, lens, width, prefix):  # noqa: 
     kp, vp = (rn(20, page, Hkv, hd).half() for _ in range(2))
     ang = torch.arange(100, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(hd // 2, dtype=torch.float64) / (hd // 2))
     _run_append(q4b, (b, q, k, v, kp, vp, ang.cos().float().to(DEV), ang.sin().float().to(DEV)), "half", page, "float16")
+
+
+# ---- prefix_attention: the same lengths -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens,width,prefix,H,Hkv,hd,page", [
+    ([(1, 33), (4, 34), (3, 50), (2, 20)], 4, 0, 8, 2, 64, 8),
+    ([(1, 33), (4, 34), (3, 50), (2, 20)], 4, 21, 8, 2, 32, 20),  # the wide kernel
+    ([(40, 70), (100, 300), (3, 2**31 - 1)], 4, 100, 4, 2, 128, 16),  # the tensor cores: rows across the table's end
+    ([(2, 2), (1, 9)], 0, 5, 2, 2, 128, 16),
+    ([(70, -3), (3, -2**31), (2, 1)], 3, 0, 4, 2, 64, 16),
+    ([(1, 40)] * 150, 2, 4500, 8, 4, 64, 16),
+])
+def test_attend_keys_behind_the_table(q4b, lens, width, prefix, H, Hkv, hd, page):  # noqa: F811
+    """Row j sees the own keys 0 .. seq_lens - n + j that the table holds, whatever seq_lens is."""
+    rng = np.random.default_rng(width)
+    pages = len(lens) * width + -(-prefix // page) + 1
+    ids = rng.permutation(pages).astype(np.int32)
+    rows = sum(n for n, _ in lens)
+    g = torch.Generator(device=DEV).manual_seed(width)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV).half()  # noqa: E731
+    q, kp, vp = rn(rows, H, hd), rn(pages, page, Hkv, hd), rn(pages, page, Hkv, hd)
+    b = dict(q_start=np.concatenate([[0], np.cumsum([n for n, _ in lens])]).astype(np.int32), prefix_len=prefix, rows=rows,
+             seq_lens=np.array([o for _, o in lens], dtype=np.int32),
+             page_table=ids[:len(lens) * width].reshape(len(lens), width), prefix_pages=ids[len(lens) * width:pages - 1])
+    d = _dev(b)
+    got = _f64(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"]))
+    # the 64-bit form counts keys up to seq_lens: columns without a page behind the table, up to where the last row looks
+    far = width * page + rows + 1
+    wide = np.concatenate([b["page_table"], np.full((len(lens), -(-far // page) - width), -1, dtype=np.int32)], 1)
+    long = np.minimum(b["seq_lens"], far)  # beyond this every row sees all that the table holds
+    ref = R.attention(_f64(q), _f64(kp), _f64(vp), dict(b, page_table=wide, seq_lens=np.maximum(long, 0)), page)
+    _check_attend(got.reshape(ref.shape), ref, _f64(vp), torch.float16, np.ones(rows, dtype=bool))
