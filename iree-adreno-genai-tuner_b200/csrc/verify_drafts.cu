@@ -5,8 +5,7 @@
 //   w = max(p - d, 0) of that row (p of the last row if all were kept): the first j with W_j > u W_{V-1}, W the
 //   running sum of w.
 //
-// The sums have 40 bits and more (64-bit words where it matters, pairs of fp32 words over the values of a
-// lane): a running sum of 10^5 probabilities in fp32 is off by more than a typical w, and the
+// The sums have 40 bits and more (64-bit words, and pairs of fp32 words over 16 values at a time): a running sum of 10^5 probabilities in fp32 is off by more than a typical w, and the
 // drawn index would depend on the order of the sum. The products u d of the tests are exact in 64 bits.
 //
 // Bound by memory: one row of p, and of d where a draft was rejected, per sequence; the acceptance tests read
@@ -75,18 +74,27 @@ __device__ __forceinline__ void unpack16(const uint4& v, float (&x)[N]) {
   }
 }
 
-// A sum in two fp32 words. The error of an fp32 addition or subtraction is itself an fp32 number, found by
-// Dekker's fast two-sum (of numbers a >= b >= 0, s = a + b: b - (s - a), and s = a - b: (a - s) - b); the errors
-// are added up in `lo`. Over a lane's few hundred values hi + lo is off by less than 2^-40 of the sum, far
-// below the share of one token, at fp32 speed: conversions to 64 bits and 64-bit additions for every value
-// took three times as long as the row's read.
+// A sum in two fp32 words, emptied into 64 bits after every kFlush values. The error of an fp32 addition or subtraction is
+// itself an fp32 number, found by Dekker's fast two-sum (of numbers a >= b >= 0, s = a + b: b - (s - a), and s = a - b:
+// (a - s) - b); the errors are added up in `lo`, which rounds too. With u = 2^-24 and S the sum of n values, an error is
+// at most u S, those of the differences together u S, so |lo| <= (k + 1) u S after k values, and the roundings of lo and of
+// its addends together u^2 S (n^2 / 2 + 5 n / 2 + 1): 169 u^2 S < 2^-40 S for n = 16. (Not emptied, over the 2048 values a lane
+// that 2^20 values on 16 warps make, equal values far below one large one put the drawn index several tokens off.) Conversions to 64 bits and
+// 64-bit additions for every value took three times as long as the row's read.
+constexpr int kFlush = 16;
 struct Sum2 {
+  double sum = 0.0;
   float hi = 0.0f, lo = 0.0f;
   float top = 0.0f;  // largest value met: an infinite one sends the piece to the careful sum
   __device__ __forceinline__ void add(float x, float e) {  // x >= 0
     const float a = fmaxf(hi, x), b = fminf(hi, x);
     hi = __fadd_rn(a, b);
     lo = __fadd_rn(lo, __fadd_rn(__fsub_rn(b, __fsub_rn(hi, a)), e));
+  }
+  __device__ __forceinline__ void flush() {
+    top = fmaxf(top, hi);
+    sum += (double)hi + (double)lo;
+    hi = lo = 0.0f;
   }
   __device__ __forceinline__ void add_target(float p) {
     p = fmaxf(p, 0.0f);  // NaN and negative: zero
@@ -121,10 +129,11 @@ struct Row {
   }
 };
 
-// A lane's share of the weights of vectors [lo, hi), every 32nd; four or eight 16-byte loads in flight.
+// A lane's share of the weights of vectors [lo, hi), every 32nd; four 16-byte loads (p's, and d's) in flight.
 template <typename T, bool REST>
 __device__ __forceinline__ double lane_sum(const Weights<T>& w, int head, int lo, int hi, int lane) {
   constexpr int N = 16 / sizeof(T), U = 4;
+  static_assert(U * N % kFlush == 0, "nothing is left in the fp32 words at the end");
   const T* p = w.p + head;
   const T* d = REST ? w.d + head : nullptr;
   Sum2 sum;
@@ -151,15 +160,16 @@ __device__ __forceinline__ double lane_sum(const Weights<T>& w, int head, int lo
 #pragma unroll
         for (int i = 0; i < N; ++i) sum.add_target(at == (unsigned)i ? 0.0f : a[i]);
       }
+      if ((u + 1) * N % kFlush == 0) sum.flush();
     }
   }
-  if (!(sum.top < INFINITY && sum.hi < INFINITY)) {  // an infinite value counts as zero
+  if (!(sum.top < INFINITY)) {  // an infinite value counts as zero
     double s = 0.0;
     for (int v = lo + lane; v < hi; v += 32)
       for (int i = 0; i < N; ++i) s += w.at(head + v * N + i);
     return s;
   }
-  return (double)sum.hi + (double)sum.lo;
+  return sum.sum;
 }
 
 __device__ __forceinline__ double warp_sum(double v) {

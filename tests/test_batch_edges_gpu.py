@@ -112,3 +112,48 @@ def test_attend_keys_behind_the_table(q4b, lens, width, prefix, H, Hkv, hd, page
     long = np.minimum(b["seq_lens"], far)  # beyond this every row sees all that the table holds
     ref = R.attention(_f64(q), _f64(kp), _f64(vp), dict(b, page_table=wide, seq_lens=np.maximum(long, 0)), page)
     _check_attend(got.reshape(ref.shape), ref, _f64(vp), torch.float16, np.ones(rows, dtype=bool))
+
+
+# ---- verify_drafts: sums of many values -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("drafts,batch", [(False, 190), (True, 150)])
+def test_verify_sums_do_not_drift(q4b, drafts, batch):  # noqa: F811
+    """The largest vocabulary with few CTAs a sequence: 256 large weights in the first half, equal ones of 2^-24.3 of
+    those everywhere, half of the mass at the very end. All weights are whole multiples of 2^-48, so that the running
+    sums are exact in 64-bit integers; the numbers lie so that the marks fall between the two, at least 2^-38 of the sum away
+    from the next border."""
+    V, unit = 1 << 20, 2.0**-48
+    per = 2 if drafts else 1
+    target = torch.zeros(batch * per, V, device=DEV)
+    draft = torch.zeros(batch * per, V, device=DEV) if drafts else None
+    uniforms = torch.zeros(batch * per)
+    want = []
+    rng = np.random.default_rng(5)
+    for b in range(batch):
+        w = torch.full((V,), 54613 + 8 * b, dtype=torch.int64, device=DEV)
+        w.view(16, -1)[:8, :128:4] = 1 << 40
+        w[-1] = 1 << 48
+        p = w.clone()
+        if drafts:  # p - d is w; the draft 5 has no target probability
+            w[5] = p[5] = 0
+            d = torch.where(w < 1 << 20, 1 << 16, 0)
+            p = p + d
+            p[5], d[5] = 0, 1 << 16
+            draft[b * per] = (d.double() * unit).float()
+        target[b * per] = (p.double() * unit).float()
+        acc = torch.cumsum(w, 0).cpu().numpy()
+        total = int(acc[-1])
+        while True:
+            k = int(int(acc[rng.integers(V // 2 + 1000, V - 1000)]) * 2**24 / total)
+            mark = k * total >> 24
+            j = int(np.searchsorted(acc, mark, side="right"))
+            if min(mark - int(acc[j - 1]), int(acc[j]) - mark) > total >> 38 and V // 2 < j < V - 1:
+                break
+        uniforms[b * per + per - 1] = k / 2**24
+        want.append(j)
+    tokens = torch.full((batch * per,), 5, dtype=torch.int32, device=DEV)
+    q_start = torch.arange(0, batch * per + 1, per, dtype=torch.int32, device=DEV)
+    got, acc = q4b.verify_drafts(target, draft, tokens, uniforms.to(DEV), q_start)
+    assert acc.tolist() == [0] * batch
+    assert got.view(batch, per)[:, 0].tolist() == want
