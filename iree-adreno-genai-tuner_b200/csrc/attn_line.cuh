@@ -2,6 +2,8 @@
 // cursors. TR rows (tokens x heads of a KV head's group) per row tile, TK keys per unit.
 #pragma once
 
+#include <type_traits>
+
 #include "paged.cuh"
 #include "prefix_attn.h"
 
@@ -23,6 +25,13 @@ __device__ __forceinline__ int cta_of(int u, int units, int ctas) {
   while ((long long)(c + 1) * units <= n) ++c;
   return c;
 }
+
+// Weights are rounded to the cache's type for the PV product. fp16 ends at 2^-24: beside one large weight the small ones of a
+// long context would be lost, all of them (40,000 keys of weight 2^-26 make 6e-4 of the result). So a kernel whose weights are
+// at most 2^SLACK multiplies them by the power of two that brings them up to 2^15, and leaves its maxima that much smaller.
+// What is then lost to fp16's end is less than 2^(SLACK - 40) of the largest weight a key.
+template <typename T, int SLACK>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.0f - SLACK : 0.0f;
 
 // Per sequence, in shared memory; every value bounded.
 struct BatchTable {

@@ -25,7 +25,7 @@
 // copies, each warp 16 rows against all keys; items of up to 16 rows split the keys instead.
 //
 // P is rounded to the cache's type for the PV product: its error, half a step per weight, averages out over
-// the keys and stays below the output's own rounding.
+// the keys and stays below the output's own rounding (fp16 ends early: kLift).
 #include <algorithm>
 #include <type_traits>
 
@@ -191,7 +191,7 @@ struct Wide {
       const float ref = mx[i] == -INFINITY ? 0.0f : mx[i];  // nothing seen yet: every weight below is exp2(-inf)
       f[i] = ex2(m[i] - ref);
       m[i] = mx[i];
-      mx[i] = ref;
+      mx[i] = ref - kLift<T, 0>;
       l[i] *= f[i];
     }
 #pragma unroll
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_wide_kernel(Pr
           float* op = d.o + row * HD + 2 * (lane & 3);
 #pragma unroll
           for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(op + 8 * n) = make_float2(w.o[n][2 * e], w.o[n][2 * e + 1]);
-          if ((lane & 3) == 0) d.ml[row] = make_float2(w.m[e], w.l[e]);
+          if ((lane & 3) == 0) d.ml[row] = make_float2(w.m[e] - kLift<T, 0>, w.l[e]);
         }
       }
     } else {
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_wide_kernel(Pr
         }
         const long long row = d.row(r);
         d.o[row * HD + e] = o;
-        if (e == 0) d.ml[row] = make_float2(mm, l);
+        if (e == 0) d.ml[row] = make_float2(mm - kLift<T, 0>, l);
       }
     }
     if (i + 1 < count) {
@@ -559,8 +559,8 @@ struct Narrow {
         f[n][e] = ex2(m[n][e] - ref);
         moved |= f[n][e] != 1.0f;
         m[n][e] = mx;
-        s[n][e] = ex2(s[n][e] - ref);
-        s[n][2 + e] = ex2(s[n][2 + e] - ref);
+        s[n][e] = ex2(s[n][e] - (ref - kLift<T, 0>));
+        s[n][2 + e] = ex2(s[n][2 + e] - (ref - kLift<T, 0>));
         l[n][e] = fmaf(l[n][e], f[n][e], s[n][e] + s[n][2 + e]);
       }
     }
@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
         const long long row = d.row(r);
         *reinterpret_cast<float4*>(d.o + row * HD + e) = o;
         // a row whose work gave up is NaN
-        if (e == 0) d.ml[row] = make_float2(mm, *fail ? __int_as_float(0x7fffffff) : l);
+        if (e == 0) d.ml[row] = make_float2(mm - kLift<T, 0>, *fail ? __int_as_float(0x7fffffff) : l);
       }
       if (i + 1 < count) {
         fence_async_smem();

@@ -13,7 +13,7 @@
 // one's softmax runs, the tensor core works for the other, and both use every K and V tile that comes in. The
 // next item's Q and first product overlap the end of the item before.
 //
-// m moves only when a row's maximum outgrows it by 2^8, which keeps P below 256 and spares most tiles the pass over
+// m moves only when a row's maximum outgrows it by 2^8, which keeps P below 256 (times kLift) and spares most tiles the pass over
 // O; exactness is not affected (l and O carry the same factor). P is rounded to the cache's type, as in
 // the other kernel. Masks (the end of the keys, causal rows, pages that do not exist) cost only where a tile has
 // any: scores by selection, and V by zeros written over the tile where some row may not see a key, since
@@ -45,7 +45,7 @@ constexpr int kTcThreads = 384;
 constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 80;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kTcThreads * kRegsLaunch, "setmaxnreg draws on the block's own registers");
 constexpr int kHalf = kTcRows / 2;  // rows of one softmax group and MMA
-constexpr float kSlack = 8.0f;  // base-2 growth of a row's maximum that its reference tolerates
+constexpr int kSlack = 8;  // base-2 growth of a row's maximum that its reference tolerates
 
 __device__ unsigned g_prefix_status = 0;
 
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        const float ref = m == -INFINITY ? 0.0f : m;
+        const float ref = (m == -INFINITY ? 0.0f : m) - kLift<T, kSlack>;
         const uint64_t scale = pair(a.scale2, a.scale2), off = pair(-ref, -ref);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      if (on) d.ml[at] = make_float2(m, l);
+      if (on) d.ml[at] = make_float2(m - kLift<T, kSlack>, l);
       tc_fence_before();  // O has been read: the next item's first PV waits for this half's P
       tiles += n;
       if (n > 0) x += n + 1, ++items;

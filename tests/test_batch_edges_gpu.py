@@ -157,3 +157,37 @@ def test_verify_sums_do_not_drift(q4b, drafts, batch):  # noqa: F811
     got, acc = q4b.verify_drafts(target, draft, tokens, uniforms.to(DEV), q_start)
     assert acc.tolist() == [0] * batch
     assert got.view(batch, per)[:, 0].tolist() == want
+
+
+# ---- prefix_attention: many small weights beside a large one ---------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,prefix,H,Hkv,hd,page", [
+    ([(1, 40000), (1, 9000)], 0, 4, 1, 128, 16),  # the narrow kernel, 8 and 16 rows
+    ([(3, 40000), (2, 30000)], 0, 8, 2, 64, 16),
+    ([(2, 40000)], 0, 8, 2, 64, 20),  # the wide kernel: keys shared by the warps, and rows
+    ([(30, 40000)], 0, 4, 2, 32, 16),
+    ([(1, 1)] * 40, 40000, 8, 2, 128, 16),  # the tensor-core kernel: the prefix, and own keys
+    ([(30, 40000)], 0, 16, 2, 64, 16),
+    ([(1, 20000)] * 3, 40000, 6, 3, 128, 128),  # parts of both
+])
+def test_small_weights_count(q4b, lens, prefix, H, Hkv, hd, page, dtype):  # noqa: F811
+    """The first key has all but a thousandth of the weight, and V of zero; each of the others 2^-26 of it, and V of one. The
+    result, N 2^-26 / (1 + N 2^-26) of the N others a row sees, is made of weights that fp16 cannot hold beside 1."""
+    n_pages = -(-prefix // page) + sum(-(-o // page) for _, o in lens)
+    b = R.make_batch(lens, page, n_pages, prefix_len=prefix)
+    kp = torch.zeros(n_pages, page, Hkv, hd, dtype=dtype, device=DEV)
+    vp = torch.ones_like(kp)
+    for first in ([b["prefix_pages"][0]] if prefix else [t[0] for t in b["page_table"]]):
+        kp[first, 0, :, 0] = 26.0
+        vp[first, 0] = 0.0
+    q = torch.zeros(b["rows"], H, hd, dtype=dtype, device=DEV)
+    q[:, :, 0] = 1.0
+    d = _dev(b)
+    got = _f64(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"],
+                                    scale=float(np.log(2.0))))
+    others = np.array([prefix + o - n + j for n, o in lens for j in range(n)], dtype=np.float64) * 2.0**-26
+    want = np.broadcast_to((others / (1 + others))[:, None], got.shape)
+    # one rounding of the result; weights are powers of two, exact in either type; exponentials and sums in fp32
+    assert (np.abs(got - want) <= (torch.finfo(dtype).eps / 2 + 2.0**-15) * want).all(), np.abs(got / want - 1).max()
