@@ -2,7 +2,7 @@
 // output and workspace allocations and the call into libq4b.so, without per-argument Python work. A step of
 // single tokens runs for a few microseconds on the GPU; the same checks in Python with ctypes took 50-65 us of host time
 // a call, this module takes a few. Refused arguments raise ValueError; a library error comes back as its
-// negative code, which the Python side turns into Q4BError with the library's message.
+// negative code, which the Python side turns into Q4BError with the library's message; torch's errors keep their types.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -10,6 +10,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -144,10 +145,8 @@ PyObject* guarded(Py_ssize_t given, Py_ssize_t wanted, const char* what, F&& f) 
     return f(c);
   } catch (const Refuse& e) {
     PyErr_SetString(PyExc_ValueError, e.why.c_str());
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
-  } catch (...) {
-    PyErr_SetString(PyExc_RuntimeError, what);
+  } catch (...) {  // torch's own, with their types: torch.OutOfMemoryError from an allocation among them
+    if (!PyErr_Occurred()) torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }

@@ -191,3 +191,26 @@ def test_small_weights_count(q4b, lens, prefix, H, Hkv, hd, page, dtype):  # noq
     want = np.broadcast_to((others / (1 + others))[:, None], got.shape)
     # one rounding of the result; weights are powers of two, exact in either type; exponentials and sums in fp32
     assert (np.abs(got - want) <= (torch.finfo(dtype).eps / 2 + 2.0**-15) * want).all(), np.abs(got / want - 1).max()
+
+
+# ---- the torch bindings -----------------------------------------------------------------------------------
+
+
+def test_out_of_memory_is_torchs(q4b):  # noqa: F811
+    """A workspace or a result that does not fit raises torch.OutOfMemoryError, which a server catches to split its step."""
+    b, q, kp, vp = _attend_case([(256, 256)] * 4, 16, 64, 64, 8, 128, torch.float16, 3)
+    d = _dev(b)
+    call = lambda **kw: q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 64, d["page_table"], d["seq_lens"], d["q_start"], **kw)  # noqa: E731
+    ref = call()
+    big = torch.empty(1, 8, 128, dtype=torch.float16, device=DEV).expand(100_000, 8, 128)  # its result: more than torch keeps
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.0)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            call(out=ref)
+        with pytest.raises(torch.OutOfMemoryError):
+            q4b.paged_rope_append(big, big, big, kp, vp, d["page_table"], d["seq_lens"], d["q_start"])
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert torch.equal(call(), ref)
