@@ -133,6 +133,12 @@ struct Call {
       refuse(std::string(name) + " must be a contiguous tensor of the result's shape and type");
     return *t;
   }
+  // Tensors that a call wrote in place count it, so that autograd notices if it had saved one (inference tensors hold no count).
+  static void wrote(PyObject* o) {
+    if (o == Py_None) return;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
   void* stream() const { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
 };
 
@@ -192,6 +198,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       c.size32(rows, "q"), c.size32(heads, "q"), rot ? static_cast<const float*>(cos->data_ptr()) : nullptr,
                       rot ? static_cast<const float*>(sin->data_ptr()) : nullptr, ts, table_rows, rot, inter, &b, &kv,
                       out.data_ptr(), c.stream());
+      if (!rc)
+        for (int i : {3, 4, 12}) c.wrote(a[i]);
     }
     return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
   });
@@ -227,6 +235,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       rc = api.attention(q->data_ptr(), r > 1 ? q->stride(0) : 0, h > 1 ? q->stride(1) : 0, r, h, (float)scale,
                          static_cast<const int32_t*>(pages->data_ptr()), &b, &kv, out.data_ptr(), ws.data_ptr(), bytes,
                          c.stream());
+      if (!rc) c.wrote(a[9]);
     }
     return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
   });
@@ -259,6 +268,7 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       static_cast<int32_t*>(out.data_ptr()), static_cast<int32_t*>(accepted.data_ptr()), c.stream());
     }
     if (rc) return PyLong_FromLong(rc);
+    c.wrote(a[5]);
     PyObject* pair = PyTuple_New(2);
     if (!pair) return nullptr;
     PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(out));

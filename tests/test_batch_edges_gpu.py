@@ -214,3 +214,34 @@ def test_out_of_memory_is_torchs(q4b):  # noqa: F811
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert torch.equal(call(), ref)
+
+
+def test_in_place_writes_are_counted(q4b):  # noqa: F811
+    """What a call writes in place has a new version, so that autograd refuses a tensor that it had saved; tensors made in
+    inference mode are taken as well."""
+    b, q, kp, vp = _attend_case([(2, 9), (1, 30)], 16, 20, 4, 2, 64, torch.float16, 3)
+    d = _dev(b)
+    meta = (d["page_table"], d["seq_lens"], d["q_start"])
+    k, v = torch.randn(2, 3, 2, 64, device=DEV).half()
+    leaf = torch.ones((), device=DEV, requires_grad=True)
+    loss = (leaf * kp.nan_to_num(0, 0, 0)).sum() + (leaf * kp).sum()
+    for out in (None, torch.empty_like(q)):
+        before = (kp._version, vp._version, q._version, k._version) + (() if out is None else (out._version,))
+        q4b.paged_rope_append(q, k, v, kp, vp, *meta, prefix_len=20, q_out=out)
+        after = (kp._version, vp._version, q._version, k._version) + (() if out is None else (out._version,))
+        assert [y - x for x, y in zip(before, after)] == [1, 1, 0, 0] + ([] if out is None else [1])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    out = torch.empty(3, 256, dtype=torch.float16, device=DEV)
+    version = out._version
+    q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 20, *meta, out=out)
+    assert out._version == version + 1
+    probs, toks = torch.softmax(torch.randn(3, 50, device=DEV), -1), torch.zeros(3, dtype=torch.int32, device=DEV)
+    new = torch.empty(3, dtype=torch.int32, device=DEV)
+    version = new._version
+    q4b.verify_drafts(probs, None, toks, torch.rand(3, device=DEV), d["q_start"], out=new)
+    assert new._version == version + 1
+    with torch.inference_mode():
+        kp2, vp2, out2 = kp.clone(), vp.clone(), torch.empty_like(out)
+    q4b.paged_rope_append(q, k, v, kp2, vp2, *meta, prefix_len=20)
+    assert torch.equal(q4b.prefix_attention(q, kp2, vp2, d["prefix_pages"], 20, *meta, out=out2), out)
