@@ -8,6 +8,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -53,6 +54,8 @@ struct Call {
     if (!THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!t.is_cuda()) refuse(std::string(name) + " must be a CUDA tensor (there is no CPU path)");
+    if (t.requires_grad() && c10::GradMode::is_enabled())
+      refuse(std::string(name) + " requires grad, and there is no backward pass: detach it, or call under torch.no_grad()");
     if (device.index() < 0)
       device = t.device();
     else if (t.device() != device)

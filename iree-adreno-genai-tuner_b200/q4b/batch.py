@@ -6,7 +6,8 @@ q_start[b + 1] - 1 of the step and, after the step, seq_lens[b] keys of its own,
 behind ``prefix_len`` keys that all sequences share. Row j of b is key s = seq_lens[b] - n_b + j at position
 prefix_len + s. Rows behind q_start[-1] (a padded step) are left as they were. Every op runs on the
 current stream of the tensors' device and can be captured into a CUDA graph, which then follows
-what the tensors hold at replay."""
+what the tensors hold at replay. There is no backward pass: tensors that require grad are refused unless
+gradients are off (``torch.no_grad()``)."""
 
 from __future__ import annotations
 

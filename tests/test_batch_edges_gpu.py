@@ -245,3 +245,23 @@ def test_in_place_writes_are_counted(q4b):  # noqa: F811
         kp2, vp2, out2 = kp.clone(), vp.clone(), torch.empty_like(out)
     q4b.paged_rope_append(q, k, v, kp2, vp2, *meta, prefix_len=20)
     assert torch.equal(q4b.prefix_attention(q, kp2, vp2, d["prefix_pages"], 20, *meta, out=out2), out)
+
+
+def test_gradients_are_not_lost_silently(q4b):  # noqa: F811
+    b, q, kp, vp = _attend_case([(2, 9), (1, 30)], 16, 20, 4, 2, 64, torch.float16, 3)
+    d = _dev(b)
+    meta = (d["page_table"], d["seq_lens"], d["q_start"])
+    k = torch.randn(3, 2, 64, device=DEV).half()
+    probs, toks, u = torch.softmax(torch.randn(3, 50, device=DEV), -1), torch.zeros(3, dtype=torch.int32, device=DEV), torch.rand(3, device=DEV)
+    grad = lambda t: t.detach().clone().requires_grad_()  # noqa: E731
+    calls = [lambda: q4b.paged_rope_append(q, grad(k), k, kp, vp, *meta, prefix_len=20),
+             lambda: q4b.prefix_attention(grad(q), kp, vp, d["prefix_pages"], 20, *meta),
+             lambda: q4b.verify_drafts(grad(probs), None, toks, u, d["q_start"])]
+    for call in calls:
+        with pytest.raises(ValueError, match="requires grad"):
+            call()
+        with torch.no_grad():
+            call()
+    ref = q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 20, *meta)
+    with torch.no_grad():
+        assert torch.equal(q4b.prefix_attention(grad(q), kp, vp, d["prefix_pages"], 20, *meta), ref)
