@@ -266,7 +266,7 @@ void q4b_prefix_attention_wait_limit(unsigned long long ns);
  * count as zero, a draft outside [0, vocab) is not kept, and weights that are all zero give the token -1.
  * out_tokens [rows]: at b's rows the kept drafts, the drawn token, then -1; accepted [batch] = n_b (0 for a
  * sequence without rows). dtype of target and draft: Q4B_F32, Q4B_F16 or Q4B_BF16; rows target_stride /
- * draft_stride elements apart. vocab <= 2^20. */
+ * draft_stride elements apart. vocab <= 2^20. The results may not overlap tokens, uniforms or q_start. */
 int q4b_verify_drafts(const void* target, const void* draft, int dtype, long long target_stride,
                       long long draft_stride, int vocab, const int32_t* tokens, const float* uniforms, int rows,
                       const int32_t* q_start, int batch, int32_t* out_tokens, int32_t* accepted, q4b_stream_t stream);

@@ -23,6 +23,12 @@ int check_launch(const char* what);
 
 inline cudaStream_t as_stream(q4b_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
+// whether [a, a + an) and [b, b + bn) share bytes
+inline bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return an && bn && x < y + bn && y < x + an;
+}
+
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // Programmatic dependent launch is on unless the environment sets Q4B_PDL=0 (read once).

@@ -389,6 +389,13 @@ extern "C" int q4b_verify_drafts(const void* target, const void* draft, int dtyp
     return set_error(Q4B_EINVAL, "%s: rows overlap (stride below vocab)", what);
   const size_t size = dtype == Q4B_F32 ? 4 : 2;
   if (!aligned(target, size) || !aligned(draft, size)) return set_error(Q4B_EINVAL, "%s: misaligned probabilities", what);
+  // other CTAs and warps read a sequence's tokens, numbers and offsets while its results are written
+  const size_t n = 4 * (size_t)rows, nb = 4 * (size_t)batch;
+  for (const void* in : {(const void*)tokens, (const void*)uniforms})
+    if (overlap(in, n, out_tokens, n) || overlap(in, n, accepted, nb))
+      return set_error(Q4B_EINVAL, "%s: the results overlap tokens or uniforms", what);
+  if (overlap(q_start, nb + 4, out_tokens, n) || overlap(q_start, nb + 4, accepted, nb) || overlap(out_tokens, n, accepted, nb))
+    return set_error(Q4B_EINVAL, "%s: the results overlap q_start or each other", what);
   VerifyArgs a;
   a.target = target, a.draft = draft;
   a.target_stride = target_stride, a.draft_stride = draft_stride;

@@ -78,7 +78,8 @@ def verify_drafts(target, draft, tokens, uniforms, q_start, *, out=None):
     bf16: row r is the distribution of the token behind row r. tokens int32 [rows]: the step's input tokens,
     the first row of a sequence its last sure token, the others its drafts. uniforms fp32 [rows] in [0, 1):
     row r decides on tokens[r + 1], a sequence's last row draws the new token. Returned at a sequence's
-    rows: its kept drafts, the drawn token, then -1; ``accepted`` counts the kept drafts.
+    rows: its kept drafts, the drawn token, then -1; ``accepted`` counts the kept drafts. ``out`` takes the tokens
+    if given; it may not be ``tokens`` itself.
 
     Draft x is kept while u * draft[x] < target[x]; the new token is drawn by inversion from the positive part
     of target - draft at the first rejected draft, or from the last row's target if all were kept."""

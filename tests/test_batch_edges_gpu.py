@@ -265,3 +265,17 @@ def test_gradients_are_not_lost_silently(q4b):  # noqa: F811
     ref = q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 20, *meta)
     with torch.no_grad():
         assert torch.equal(q4b.prefix_attention(grad(q), kp, vp, d["prefix_pages"], 20, *meta), ref)
+
+
+# ---- results over inputs ----------------------------------------------------------------------------------
+
+
+def test_verify_refuses_results_over_tokens(q4b):  # noqa: F811
+    toks, qs = torch.zeros(5, dtype=torch.int32, device=DEV), torch.tensor([0, 3, 5], dtype=torch.int32, device=DEV)
+    probs, u = torch.softmax(torch.randn(5, 50, device=DEV), -1), torch.rand(5, device=DEV)
+    with pytest.raises(q4b.Q4BError, match="overlap"):
+        q4b.verify_drafts(probs, None, toks, u, qs, out=toks)
+    both = torch.zeros(10, dtype=torch.int32, device=DEV)  # neighbours in one buffer are apart
+    a, _ = q4b.verify_drafts(probs, None, both[:5], u, qs, out=both[5:])
+    b, _ = q4b.verify_drafts(probs, None, toks, u, qs)
+    assert torch.equal(a, b)
