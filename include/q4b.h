@@ -230,7 +230,8 @@ typedef struct q4b_paged_kv {
  * rope_stride apart: row p holds position p's angles (whatever scaling they were made with). The first rot_dim
  * elements of a head turn, pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved; the rest is
  * copied. head_dim and rot_dim are multiples of 16; rot_dim 0 turns nothing (tables may be NULL).
- * q_out [rows, n_heads, head_dim] of kv->dtype. Computed in fp32, rounded once. A row whose position the
+ * q_out [rows, n_heads, head_dim] of kv->dtype; it may be q itself, contiguous and of that type, and overlaps q, k or v in
+ * no other way. Computed in fp32, rounded once. A row whose position the
  * tables do not reach gets q_out = 0 and appends nothing. Two sequences that append to one slot race. */
 int q4b_paged_rope_append(const void* q, const void* k, const void* v, int x_dtype, long long q_stride,
                           long long k_stride, long long v_stride, int rows, int n_heads, const float* rope_cos,

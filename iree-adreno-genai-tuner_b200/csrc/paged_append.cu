@@ -230,6 +230,15 @@ extern "C" int q4b_paged_rope_append(const void* q, const void* k, const void* v
   if ((long long)(n_heads + 2ll * kv->n_kv_heads) * kv->head_dim > (1 << 24))
     return set_error(Q4B_EUNSUPPORTED, "%s: more than 2^24 elements a row", what);
   if (rows == 0 || batch->batch == 0) return Q4B_OK;
+  // A task reads its 16 elements before it writes them, so q_out may be q, element for element; any other overlap is read by
+  // tasks that run after it was written.
+  const size_t size = x_dtype == Q4B_F32 ? 4 : 2, q_row = (size_t)n_heads * kv->head_dim, kv_row = (size_t)kv->n_kv_heads * kv->head_dim;
+  auto over = [&](const void* x, long long stride, size_t row) {
+    return overlap(x, ((size_t)(rows - 1) * (size_t)stride + row) * size, q_out, (size_t)rows * q_row * 2);
+  };
+  const bool in_place = q_out == q && size == 2 && (rows == 1 || q_stride == (long long)q_row);
+  if ((!in_place && over(q, q_stride, q_row)) || over(k, k_stride, kv_row) || over(v, v_stride, kv_row))
+    return set_error(Q4B_EINVAL, "%s: q_out overlaps q, k or v (it may be q itself, of the cache's type and contiguous)", what);
   AppendArgs a;
   a.q = q, a.k = k, a.v = v;
   a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;

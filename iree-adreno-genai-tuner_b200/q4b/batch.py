@@ -45,7 +45,7 @@ def paged_rope_append(q, k, v, k_pages, v_pages, page_table, seq_lens, q_start, 
     place; cos, sin fp32 [positions, rot / 2] (``rope_tables(...)[i][:, : rot // 2]``, or tables of any
     scaling): the first ``rot`` elements of a head turn, as pairs (i, i + rot / 2) with layout "half" and
     (2 i, 2 i + 1) with "interleaved"; None turns nothing. The rotated q is [rows, H, hd] of the cache's type
-    (``q_out`` if given). head_dim and rot are multiples of 16.
+    (``q_out`` if given; it may be q itself). head_dim and rot are multiples of 16.
 
     The step's rows come last in their sequences: seq_lens counts them. To fill the shared prefix itself,
     call with prefix_len = 0 and page_table = prefix_pages[None]."""

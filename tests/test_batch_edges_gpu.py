@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import batch_ref as R
-from test_batch_gpu import DEV, _attend_case, _check_attend, _dev, _f64, _run_append, _run_attend, q4b  # noqa: F401
+from test_batch_gpu import DEV, _append_case, _attend_case, _check_attend, _dev, _f64, _run_append, _run_attend, q4b  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -279,3 +279,21 @@ def test_verify_refuses_results_over_tokens(q4b):  # noqa: F811
     a, _ = q4b.verify_drafts(probs, None, both[:5], u, qs, out=both[5:])
     b, _ = q4b.verify_drafts(probs, None, toks, u, qs)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("rows,fused", [(700, False), (1, True)])
+def test_append_rotates_q_in_place(q4b, layout, rows, fused):  # noqa: F811
+    """q_out = q: contiguous, or the one row of a fused projection."""
+    b, q, k, v, kp, vp, cos, sin = _append_case([(rows, rows + 9)], 16, 3, 8, 2, 64, 32, "float16", "float16", 3)
+    d = _dev(b)
+    meta = (d["page_table"], d["seq_lens"], d["q_start"], cos, sin)
+    kw = dict(prefix_len=3, layout=layout)
+    ref = q4b.paged_rope_append(q, k, v, kp, vp, *meta, **kw)
+    k0, v0 = kp.clone(), vp.clone()
+    q2 = q if fused else q.contiguous()
+    assert q4b.paged_rope_append(q2, k, v, kp, vp, *meta, q_out=q2, **kw) is q2
+    assert torch.equal(q2, ref) and torch.equal(kp, k0) and torch.equal(vp, v0)
+    with pytest.raises(q4b.Q4BError, match="overlap"):
+        wide = torch.zeros(rows * 8 * 64 + 64, dtype=torch.float16, device=DEV)
+        q4b.paged_rope_append(wide[:-64].view(-1, 8, 64), k, v, kp, vp, *meta, q_out=wide[64:].view(-1, 8, 64), **kw)
