@@ -957,7 +957,7 @@ Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv, bool wide
   constexpr int kAll = 0x7fffffff;
   const int Hkv = kv.n_kv_heads, g = H / Hkv, R = rows * g;
   Plan p = {};
-  const bool tc = prefix_tc_takes(kv) && wide_q;
+  const bool tc = prefix_tc_takes(kv) && wide_q && prefix_tc_built(kv);
   const bool tc_prefix = tc && prefix_units(rows, g, Hkv, b.prefix_len, 16, kMmKeys) > kTcMinUnits;
   // several rows a sequence on average: those with many are worth the tensor cores
   const bool tc_own = tc && rows > b.batch && R > kTcMinRows && b.batch <= kTcMaxBatch;

@@ -617,6 +617,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
+// The registers that the kernel was compiled to; -1 where the runtime cannot tell (no device).
+template <typename T, int HD>
+int registers() {
+  static std::atomic<int> known{-1};
+  int regs = known.load(std::memory_order_relaxed);
+  if (regs < 0) {
+    cudaFuncAttributes f = {};
+    if (cudaFuncGetAttributes(&f, prefix_tc_kernel<T, HD>) == cudaSuccess)
+      known.store(regs = f.numRegs, std::memory_order_relaxed);
+    else
+      cudaGetLastError();
+  }
+  return regs;
+}
+
 template <typename T, int HD>
 int launch(const PrefixArgs& a, cudaStream_t st) {
   CUtensorMap tk, tv;
@@ -625,12 +640,8 @@ int launch(const PrefixArgs& a, cudaStream_t st) {
   if (int rc = make_tmap_pages(&tv, a.kv, a.kv.v, box)) return rc;
   auto kern = prefix_tc_kernel<T, HD>;
   static std::atomic<unsigned long long> done;
-  // the register split needs the launch registers that it was laid out for
-  static const int regs = [&] {
-    cudaFuncAttributes f = {};
-    return cudaFuncGetAttributes(&f, kern) == cudaSuccess ? f.numRegs : 0;
-  }();
-  if (regs != kRegsLaunch) return set_error(Q4B_EUNSUPPORTED, "prefix_attention: built with %d registers, not %d", regs, kRegsLaunch);
+  if (const int regs = registers<T, HD>(); regs != kRegsLaunch)  // the plan asked already, unless the runtime could not tell then
+    return set_error(Q4B_EUNSUPPORTED, "prefix_attention: built with %d registers, not %d", regs, kRegsLaunch);
   const int table = a.tc.own_lo < a.tc.own_hi ? 12 * (a.b.batch + 1) : 0;
   cudaError_t e = set_max_dynamic_smem(kern, TcCfg<HD>::SMEM + 12 * (kTcMaxBatch + 1), done);
   if (e == cudaSuccess) e = launch_pdl(kern, dim3(a.tc_ctas), dim3(kTcThreads), TcCfg<HD>::SMEM + table, st, tk, tv, a);
@@ -647,6 +658,15 @@ int launch(const PrefixArgs& a, cudaStream_t st) {
 bool prefix_tc_takes(const q4b_paged_kv& kv) {
   const bool strides = kv.slot_stride > 0 && (kv.n_kv_heads == 1 || kv.head_stride > 0) && (kv.n_pages == 1 || kv.page_stride > 0);
   return kv.head_dim >= 64 && kv.page_size % 8 == 0 && strides;
+}
+
+// The register split (setmaxnreg) needs the launch registers that it was laid out for: a compiler that gives the kernel others
+// leaves all items to the other kernels.
+bool prefix_tc_built(const q4b_paged_kv& kv) {
+  const bool h16 = kv.dtype == Q4B_F16;
+  const int regs = kv.head_dim == 128 ? (h16 ? registers<__half, 128>() : registers<__nv_bfloat16, 128>())
+                                      : (h16 ? registers<__half, 64>() : registers<__nv_bfloat16, 64>());
+  return regs < 0 || regs == kRegsLaunch;
 }
 
 int prefix_tc_run(const PrefixArgs& a, cudaStream_t st) {

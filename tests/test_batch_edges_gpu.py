@@ -297,3 +297,32 @@ def test_append_rotates_q_in_place(q4b, layout, rows, fused):  # noqa: F811
     with pytest.raises(q4b.Q4BError, match="overlap"):
         wide = torch.zeros(rows * 8 * 64 + 64, dtype=torch.float16, device=DEV)
         q4b.paged_rope_append(wide[:-64].view(-1, 8, 64), k, v, kp, vp, *meta, q_out=wide[64:].view(-1, 8, 64), **kw)
+
+
+# ---- prefix_attention: which kernels run ------------------------------------------------------------------
+
+
+def _kernels(call):
+    from torch.profiler import ProfilerActivity, profile
+    call()
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as prof:
+        call()
+        torch.cuda.synchronize()
+    return [e.key for e in prof.key_averages() if "prefix_" in e.key]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_rows_run_on_the_tensor_core_kernel(q4b, hd, dtype):  # noqa: F811
+    """In this build the tensor-core kernel has the registers of its split, so the plan uses it; and a step that it is not
+    used for (here for its q) runs on the other kernels with the same results."""
+    b, q, kp, vp = _attend_case([(20, 70), (30, 40), (1, 8)], 16, 6000, 16, 8, hd, dtype, 5)
+    d = _dev(b)
+    odd = torch.empty(b["rows"], 16 * hd + 2, dtype=dtype, device=DEV)[:, 2:].view(b["rows"], 16, hd)
+    odd.copy_(q)
+    call = lambda x: q4b.prefix_attention(x, kp, vp, d["prefix_pages"], 6000, d["page_table"], d["seq_lens"], d["q_start"])  # noqa: E731
+    on, off = _kernels(lambda: call(q)), _kernels(lambda: call(odd))
+    assert any("prefix_tc_kernel" in k for k in on), on
+    assert not any("prefix_tc_kernel" in k for k in off) and any("prefix_narrow_kernel" in k for k in off), off
+    _run_attend(q4b, (b, odd, kp, vp), 16)
