@@ -211,6 +211,10 @@ typedef struct q4b_batch {
   int batch, table_width;
   long long table_stride;
   int prefix_len;
+  /* What the caller knows of a step without a look at the device, 0: not known. The attention's choice of kernels and SMs goes
+   * by them, its results do not. */
+  int max_new;  /* most rows of any sequence. Not known: 1 if rows <= batch, so a prompt chunk among idle sequences wants it */
+  int own_keys; /* own keys of a sequence, about. Not known: half of what a row of the table holds, so a wide table wants it */
 } q4b_batch;
 
 /* Pools of pages [n_pages, page_size, n_kv_heads, head_dim] of fp16 or bf16 (dtype Q4B_F16 / Q4B_BF16), k

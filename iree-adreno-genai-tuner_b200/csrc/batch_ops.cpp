@@ -90,7 +90,7 @@ struct Call {
     if (qs->size(0) != n + 1 || pt->size(0) != n)
       refuse(std::to_string(n) + " seq_lens need q_start [" + std::to_string(n + 1) + "] and page_table [" +
              std::to_string(n) + ", ...]");
-    q4b_batch b;
+    q4b_batch b = {};
     b.q_start = static_cast<const int32_t*>(qs->data_ptr());
     b.seq_lens = static_cast<const int32_t*>(sl->data_ptr());
     b.page_table = static_cast<const int32_t*>(pt->data_ptr());
@@ -209,12 +209,14 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 10, "prefix_attention", [&](Call& c) -> PyObject* {
+  return guarded(n, 12, "prefix_attention", [&](Call& c) -> PyObject* {
     const at::Tensor* q = c.tensor(a[0], "q");
     at::ScalarType type;
     const q4b_paged_kv kv = c.paged_kv(a[1], a[2], type);
     const at::Tensor* pages = c.int32(a[3], "prefix_pages", 1);
-    const q4b_batch b = c.batch(a[7], a[6], a[5], a[4]);
+    q4b_batch b = c.batch(a[7], a[6], a[5], a[4]);
+    if (a[10] != Py_None) b.max_new = c.integer(a[10], "max_new");
+    if (a[11] != Py_None) b.own_keys = c.integer(a[11], "own_keys");
     if (pages->size(0) * (long long)kv.page_size < b.prefix_len)
       c.refuse(std::to_string(pages->size(0)) + " prefix pages of " + std::to_string(kv.page_size) + " hold no " +
                std::to_string(b.prefix_len) + " keys");

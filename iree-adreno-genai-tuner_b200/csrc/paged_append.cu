@@ -19,7 +19,7 @@ namespace q4b {
 
 int check_batch(const char* what, const q4b_batch* b, int rows) {
   if (!b) return set_error(Q4B_EINVAL, "%s: null batch", what);
-  if (rows < 0 || b->batch < 0 || b->table_width < 0 || b->prefix_len < 0)
+  if (rows < 0 || b->batch < 0 || b->table_width < 0 || b->prefix_len < 0 || b->max_new < 0 || b->own_keys < 0)
     return set_error(Q4B_EINVAL, "%s: negative size", what);
   if (b->prefix_len > 0x7fffff00) return set_error(Q4B_EINVAL, "%s: prefix_len %d is too large", what, b->prefix_len);
   if (!b->q_start || (b->batch > 0 && !b->seq_lens) || (b->batch > 0 && b->table_width > 0 && !b->page_table))

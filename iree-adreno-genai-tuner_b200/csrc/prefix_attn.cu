@@ -959,8 +959,10 @@ Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv, bool wide
   Plan p = {};
   const bool tc = prefix_tc_takes(kv) && wide_q && prefix_tc_built(kv);
   const bool tc_prefix = tc && prefix_units(rows, g, Hkv, b.prefix_len, 16, kMmKeys) > kTcMinUnits;
-  // several rows a sequence on average: those with many are worth the tensor cores
-  const bool tc_own = tc && rows > b.batch && R > kTcMinRows && b.batch <= kTcMaxBatch;
+  // several rows a sequence, as told or on average: those with many are worth the tensor cores
+  const bool several = b.max_new ? b.max_new > 1 : rows > b.batch;
+  const int most_rows = several ? (b.max_new ? std::min(b.max_new, rows) : rows) * g : g;  // of a sequence, times heads
+  const bool tc_own = tc && several && most_rows > kTcMinRows && b.batch <= kTcMaxBatch;
   if (tc_prefix || tc_own) p.tc_ctas = kTcCtas;
   if (tc_prefix) p.tc.prefix_units = prefix_units(rows, g, Hkv, b.prefix_len, kTcRows, kTcKeys);
   p.tc.own_lo = tc_own ? kTcMinRows : kAll;
@@ -968,31 +970,38 @@ Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv, bool wide
   p.mm.own_hi = tc_own ? kTcMinRows : kAll;
   // Row tiles: 8 for single tokens, 16 for a few rows; more rows are more tiles, whose keys come from L2 again.
   const bool prefix_here = !tc_prefix && b.prefix_len > 0;
-  const int most = std::max(rows > b.batch ? R : g, prefix_here ? R : 0);
+  const int most = std::max(most_rows, prefix_here ? R : 0);
   p.mm_rows = !prefix_tc_takes(kv) ? 64 : most <= 8 ? 8 : 16;
   if (prefix_here) p.mm.prefix_units = prefix_units(rows, g, Hkv, b.prefix_len, p.mm_rows, kMmKeys);
   int mm_sms = kSms;
   // Small steps, where either kernel's start and end (some 10 us of launch, first reads and last parts) weigh as much as
   // its tiles: both at once, on disjoint SMs, instead of one behind the other. 61 sequences of 5 drafts behind 4099 keys: 45
-  // us against 52; 192 single tokens behind 16384 keys, where a wrong guess at the own keys (0.6 of what the page tables
-  // hold) costs more than the start: 207 at best against 210.
+  // us against 52; 192 single tokens behind 16384 keys, where a wrong guess at the own keys costs more than the start: 207 at
+  // best against 210. Where the caller does not tell them, own keys are anything from none to full tables, and what counts is the
+  // mean over four lengths between.
   const int per_sequence = (R + std::max(b.batch, 1) - 1) / std::max(b.batch, 1);
   const int items = Hkv * ((R + kTcRows - 1) / kTcRows);
   if (tc_prefix && per_sequence <= kTcMinRows && p.mm_rows < 64) {
     const int tiles = (b.prefix_len + kTcKeys - 1) / kTcKeys;
     const double tile_us = kv.head_dim == 128 ? 2.0 : 1.6;
     // row tiles of a sequence (ragged: a little above the mean), an item's start and end as 1.3 tiles
-    const double row_tiles = rows <= b.batch ? (per_sequence + p.mm_rows - 1) / p.mm_rows
+    const double row_tiles = !several ? (per_sequence + p.mm_rows - 1) / p.mm_rows
                                              : std::max(1.0, (double)R / std::max(b.batch, 1) / p.mm_rows + 0.2);
-    const double mm_us = b.batch * (double)Hkv * row_tiles * (0.6 * b.table_width * kv.page_size / kMmKeys + 1.3) * 1.3 /
-                         (mm_ctas_per_sm(kv.head_dim) * kSms);
+    const double full = (double)b.table_width * kv.page_size, known = std::min<double>(b.own_keys, full);
+    auto mm_time = [&](double own) {
+      return b.batch * (double)Hkv * row_tiles * (own / kMmKeys + 1.3) * 1.3 / (mm_ctas_per_sm(kv.head_dim) * kSms);
+    };
+    const double mm_us = mm_time(b.own_keys ? known : 0.5 * full);
     const double tc_us = (double)items * tiles * tile_us / kSms;
     if (tc_us + mm_us < 40) {
       // SMs for the prefix: a multiple of its items, so that no CTA has parts of two (that costs some 3 us), or the share of
       // the tiles' time. More CTAs an item are more parts for the join, 0.5 us each. Measured against the share alone: 24
       // sequences of 6 behind 3000 keys 35 us and 49, 32 single tokens behind 2048 25 and 28.5, 64 behind 1500 42.5 and 40.
       auto cost = [&](int ctas, double each, double parts) {
-        return std::max(2.0 + each * tile_us, mm_us * kSms / (kSms - ctas)) + 0.5 * parts;
+        double us = 0.0;
+        for (double f : {0.125, 0.375, 0.625, 0.875})
+          us += 0.25 * std::max(2.0 + each * tile_us, mm_time(b.own_keys ? known : f * full) * kSms / (kSms - ctas));
+        return us + 0.5 * parts;
       };
       int best = 0;
       double least = 1e30;

@@ -62,7 +62,8 @@ class LayerWeights(ctypes.Structure):
 
 class Batch(ctypes.Structure):
     _fields_ = [("q_start", c_void_p), ("seq_lens", c_void_p), ("page_table", c_void_p), ("batch", c_int),
-                ("table_width", c_int), ("table_stride", ctypes.c_longlong), ("prefix_len", c_int)]
+                ("table_width", c_int), ("table_stride", ctypes.c_longlong), ("prefix_len", c_int),
+                ("max_new", c_int), ("own_keys", c_int)]
 
 
 class PagedKV(ctypes.Structure):

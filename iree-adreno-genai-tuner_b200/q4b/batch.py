@@ -57,15 +57,19 @@ def paged_rope_append(q, k, v, k_pages, v_pages, page_table, seq_lens, q_start, 
 
 
 def prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, page_table, seq_lens, q_start, *,
-                     scale=None, out=None):
+                     scale=None, out=None, max_new=None, own_keys=None):
     """Attention of a step's rows over the shared prefix and each sequence's own keys -> [rows, H * hd].
 
     q [rows, H, hd] of the cache's type, rotated (any row and head stride); prefix_pages int32: the pages
     of the prefix_len shared keys (prefix_len 0: none, every sequence on its own). Row j of sequence b sees the
     prefix and b's own keys up to its own; a row that sees none is zero. The prefix is read
-    once for all sequences. scale defaults to 1 / sqrt(hd). head_dim 32, 64 or 128."""
+    once for all sequences. scale defaults to 1 / sqrt(hd). head_dim 32, 64 or 128.
+
+    max_new and own_keys, where the caller knows them, choose among kernels and change no result: the most rows of any
+    sequence (else 1 if rows <= B, so a step of one prompt chunk and many idle sequences wants it), and about how many
+    own keys a sequence has (else half of what a row of page_table holds, so tables much wider than the sequences want it)."""
     r = (_OPS or _ops()).prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, seq_lens, q_start,
-                                          scale, out)
+                                          scale, out, max_new, own_keys)
     if r.__class__ is int:
         check(r, "prefix_attention")
     return r

@@ -39,3 +39,30 @@ def test_append_refuses_overlapping_q_out(L, where):
     rc = L.q4b_paged_rope_append(P, a["k"], a["v"], a["x_dtype"], a["qs"], 128, 128, 3, 8, 8 * P, 9 * P, 32, 64, 64, 0,
                                  ctypes.byref(b), ctypes.byref(c), a["out"], None)
     assert rc == _lib.Q4B_EINVAL and b"overlap" in L.q4b_last_error()
+
+
+def _attend_batch(lib, **kw):
+    d = dict(q_start=P, seq_lens=P, page_table=P, batch=32, table_width=32, table_stride=8192, prefix_len=2048)
+    d.update(kw)
+    kv = dict(k=P, v=P, dtype=lib.F16, n_pages=10_000, page_size=16, n_kv_heads=8, head_dim=128, page_stride=16 * 8 * 128,
+              slot_stride=8 * 128, head_stride=128)
+    return lib.Batch(**d), lib.PagedKV(**kv)
+
+
+def test_attention_plans_by_told_lengths_not_by_the_tables_width(L):
+    """The workspace's size shows how the kernels share the SMs: the same for a table of any width if own_keys is told."""
+    from q4b import _lib
+    size = lambda **kw: L.q4b_prefix_attention_workspace(32, 24, *map(ctypes.byref, _attend_batch(_lib, **kw)))  # noqa: E731
+    told = {size(own_keys=300, table_width=w) for w in (32, 128, 512, 8192)}
+    assert len(told) == 1 and told != {0}
+    assert size(table_width=32) != size(table_width=8192)  # the width is all that is known then
+    # a prompt chunk among idle sequences: the own keys of many rows need places of the tensor-core kernel
+    assert size(prefix_len=0, max_new=20) > size(prefix_len=0)
+
+
+@pytest.mark.parametrize("bad", [dict(max_new=-1), dict(own_keys=-1)])
+def test_attention_refuses_negative_hints(L, bad):
+    from q4b import _lib
+    b, kv = _attend_batch(_lib, **bad)
+    assert L.q4b_prefix_attention_workspace(32, 24, ctypes.byref(b), ctypes.byref(kv)) == 0
+    assert b"negative" in L.q4b_last_error()

@@ -326,3 +326,36 @@ def test_many_rows_run_on_the_tensor_core_kernel(q4b, hd, dtype):  # noqa: F811
     assert any("prefix_tc_kernel" in k for k in on), on
     assert not any("prefix_tc_kernel" in k for k in off) and any("prefix_narrow_kernel" in k for k in off), off
     _run_attend(q4b, (b, odd, kp, vp), 16)
+
+
+@pytest.mark.parametrize("lens,prefix,width", [
+    ([(180, 700), (1, 90), (1, 1)] + [(0, 5)] * 190, 0, 50),  # fewer rows than sequences, most of them in one
+    ([(180, 700), (1, 90), (1, 1)] + [(0, 5)] * 190, 5000, 50),
+    ([(1, 200)] * 33, 2500, 400),  # tables much wider than the sequences
+    ([(3, 70), (5, 9), (1, 300)] * 8, 3000, 300),
+])
+def test_told_lengths_change_no_result(q4b, lens, prefix, width):  # noqa: F811
+    """max_new and own_keys, right or far off, choose kernels and SMs only."""
+    n_pages = sum(-(-o // 16) for _, o in lens) + -(-prefix // 16) + 2
+    b = R.make_batch(lens, 16, n_pages, prefix_len=prefix, width=width)
+    g = torch.Generator(device=DEV).manual_seed(width)
+    q = torch.randn(b["rows"], 16, 64, generator=g, device=DEV).half()
+    kp, vp = (torch.randn(n_pages, 16, 4, 64, generator=g, device=DEV).half() for _ in range(2))
+    most, mean = max(n for n, _ in lens), int(np.mean([o for _, o in lens]))
+    for kw in ({}, dict(max_new=most, own_keys=mean), dict(max_new=1), dict(max_new=2**31 - 1, own_keys=1),
+               dict(own_keys=2**31 - 1)):
+        d = _dev(b)
+        out = _f64(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"], **kw))
+        ref = R.attention(_f64(q), _f64(kp), _f64(vp), b, 16) if not kw else ref
+        _check_attend(out.reshape(ref.shape), ref, _f64(vp), torch.float16, np.ones(b["rows"], dtype=bool))
+    for bad in (dict(max_new=-1), dict(own_keys="x")):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"], **bad)
+
+
+def test_a_told_prompt_chunk_runs_on_the_tensor_cores(q4b):  # noqa: F811
+    b, q, kp, vp = _attend_case([(180, 700), (1, 90)] + [(0, 5)] * 190, 16, 0, 16, 4, 64, torch.float16, 5)
+    d = _dev(b)
+    call = lambda **kw: q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 0, d["page_table"], d["seq_lens"], d["q_start"], **kw)  # noqa: E731
+    assert any("prefix_tc_kernel" in k for k in _kernels(lambda: call(max_new=180)))
+    assert not any("prefix_tc_kernel" in k for k in _kernels(lambda: call(max_new=1)))
