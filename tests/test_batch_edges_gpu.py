@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import batch_ref as R
-from test_batch_gpu import DEV, _append_case, _attend_case, _check_attend, _dev, _f64, _run_append, _run_attend, q4b  # noqa: F401
+from test_batch_gpu import (DEV, _append_case, _attend_case, _check_attend, _close_rounded, _dev, _f64, _run_append,  # noqa: F401
+                            _run_attend, _verify_case, q4b)
 
 pytestmark = pytest.mark.gpu
 
@@ -359,3 +360,106 @@ def test_a_told_prompt_chunk_runs_on_the_tensor_cores(q4b):  # noqa: F811
     call = lambda **kw: q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 0, d["page_table"], d["seq_lens"], d["q_start"], **kw)  # noqa: E731
     assert any("prefix_tc_kernel" in k for k in _kernels(lambda: call(max_new=180)))
     assert not any("prefix_tc_kernel" in k for k in _kernels(lambda: call(max_new=1)))
+
+
+# ---- malformed offsets, with guards around everything that a call may write -------------------------------
+
+
+class _Guarded:
+    """A tensor inside a larger buffer of a known byte."""
+
+    def __init__(self, shape, dtype, fill=0x5A):
+        size = int(np.prod(shape)) * torch.empty((), dtype=dtype).element_size()
+        self.raw = torch.full((size + (2 << 20),), fill, dtype=torch.uint8, device=DEV)
+        self.size, self.fill = size, fill
+        self.t = self.raw[1 << 20:(1 << 20) + size].view(dtype).view(shape)
+
+    def check(self):
+        assert bool((self.raw[:1 << 20] == self.fill).all()) and bool((self.raw[(1 << 20) + self.size:] == self.fill).all())
+
+
+OFFSETS = [[0, 3, 900], [0, 5, 2], [-4, 3, 6], [9, 9, 9], [4, 4, 5], [0, 3, 6]]
+
+
+def _clamped(offsets, rows):
+    """The offsets that the operators go by: clamped to the rows; decreasing ones hold no sequence (attention)."""
+    return np.clip(np.array(offsets), 0, rows).astype(np.int32), any(b < a for a, b in zip(offsets, offsets[1:]))
+
+
+@pytest.mark.parametrize("offsets", OFFSETS)
+@pytest.mark.parametrize("rows,prefix,H,Hkv,hd,page", [(6, 50, 8, 2, 64, 8), (6, 50, 4, 2, 32, 20), (6, 30_000, 16, 4, 128, 16),
+                                                       (150, 50, 4, 2, 64, 16)])
+def test_attend_malformed_offsets_and_guards(q4b, rows, prefix, H, Hkv, hd, page, offsets):  # noqa: F811
+    """Rows of no sequence keep what out held, the others follow the clamped offsets, and nothing is written outside out and a
+    workspace of exactly the size that was asked for."""
+    import ctypes
+    from q4b import _lib
+    L = _lib.lib()
+    own = 44
+    b, q, kp, vp = _attend_case([(rows // 2, own), (rows - rows // 2, own)], page, prefix, H, Hkv, hd, torch.float16, 9)
+    offsets = [o * rows // 6 for o in offsets]
+    d = _dev(b)
+    d["q_start"] = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    width = b["page_table"].shape[1]
+    # the pool's slots behind the own keys count as keys here: finite ones
+    kp, vp = kp.nan_to_num(0.25), vp.nan_to_num(0.5, 0.5, 0.5)
+    lens = [2**31 - 1, -5]
+    d["seq_lens"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = _Guarded((rows, H * hd), torch.float16)
+    out.t.fill_(7.0)
+    batch = _lib.Batch(q_start=d["q_start"].data_ptr(), seq_lens=d["seq_lens"].data_ptr(), page_table=d["page_table"].data_ptr(),
+                       batch=2, table_width=width, table_stride=width, prefix_len=prefix)
+    kv = _lib.PagedKV(k=kp.data_ptr(), v=vp.data_ptr(), dtype=_lib.F16, n_pages=kp.shape[0], page_size=page, n_kv_heads=Hkv,
+                      head_dim=hd, page_stride=kp.stride(0), slot_stride=kp.stride(1), head_stride=kp.stride(2))
+    need = L.q4b_prefix_attention_workspace(rows, H, ctypes.byref(batch), ctypes.byref(kv))
+    ws = _Guarded((need,), torch.uint8)
+    rc = L.q4b_prefix_attention(q.data_ptr(), H * hd, hd, rows, H, hd**-0.5, d["prefix_pages"].data_ptr(), ctypes.byref(batch),
+                                ctypes.byref(kv), out.t.data_ptr(), ws.t.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, L.q4b_last_error()
+    torch.cuda.synchronize()
+    out.check(), ws.check()
+    q_start, bad = _clamped(offsets, rows)
+    if bad:
+        assert bool((out.t == 7.0).all())
+        return
+    far = width * page + rows + 1
+    wide = np.concatenate([b["page_table"], np.full((2, -(-far // page) - width), -1, dtype=np.int32)], 1)
+    ref = R.attention(_f64(q), _f64(kp), _f64(vp), dict(b, q_start=q_start, page_table=wide,
+                                                        seq_lens=np.array([min(x, far) if x > 0 else 0 for x in lens])), page)
+    live = ~np.isnan(ref).any(axis=(1, 2))
+    got = _f64(out.t).reshape(ref.shape)
+    assert (got[~live] == 7.0).all()
+    _check_attend(np.where(live[:, None, None], got, 0), np.where(live[:, None, None], ref, 0), _f64(vp), torch.float16, live)
+
+
+@pytest.mark.parametrize("offsets", OFFSETS)
+def test_append_and_verify_malformed_offsets_and_guards(q4b, offsets):  # noqa: F811
+    rows, H, Hkv, hd, page = 6, 4, 2, 64, 8
+    b, q, k, v, kp, vp, cos, sin = _append_case([(3, 30), (3, 44)], page, 0, H, Hkv, hd, 64, "float16", "float16", 9)
+    d = _dev(b)
+    q_start, bad = _clamped(offsets, rows)
+    qs = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    gk, gv, out = _Guarded(kp.shape, kp.dtype), _Guarded(vp.shape, vp.dtype), _Guarded((rows, H, hd), q.dtype)
+    gk.t.copy_(kp), gv.t.copy_(vp), out.t.fill_(7.0)
+    q4b.paged_rope_append(q, k, v, gk.t, gv.t, d["page_table"], d["seq_lens"], qs, cos, sin, q_out=out.t)
+    for x in (gk, gv, out):
+        x.check()
+    if not bad:
+        k0, v0 = _f64(kp), _f64(vp)
+        ref = R.append(_f64(q), _f64(k), _f64(v), k0, v0, dict(b, q_start=q_start), _f64(cos), _f64(sin), "half", page)
+        live = ~np.isnan(ref).any(axis=(1, 2))
+        assert (_f64(out.t)[~live] == 7.0).all()
+        _close_rounded(_f64(out.t)[live], ref[live], torch.float16, 2 * np.abs(_f64(q)).max())
+        _close_rounded(_f64(gk.t), k0, torch.float16, 2 * np.abs(_f64(k)).max())
+        _close_rounded(_f64(gv.t), v0, torch.float16, 0.0)
+    target, draft, tokens, uniforms, _ = _verify_case([3, 3], 257, torch.float32, True, 6)
+    new = _Guarded((rows,), torch.int32)
+    new.t.fill_(77)
+    _, acc = q4b.verify_drafts(target, draft, tokens, uniforms, qs, out=new.t)
+    new.check()
+    if bad:
+        assert all(0 <= a <= rows for a in acc.tolist())
+        return
+    n = lambda t: t.cpu().numpy()  # noqa: E731
+    want, kept = R.verify(n(target), n(draft), n(tokens), n(uniforms), q_start)
+    assert acc.tolist() == kept and new.t.tolist() == [77 if w is None else w for w in want]
