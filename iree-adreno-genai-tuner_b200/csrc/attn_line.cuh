@@ -32,6 +32,13 @@ __device__ __forceinline__ int cta_of(int u, int units, int ctas) {
 // What is then lost to fp16's end is less than 2^(SLACK - 40) of the largest weight a key.
 template <typename T, int SLACK>
 constexpr float kLift = std::is_same<T, __half>::value ? 15.0f - SLACK : 0.0f;
+// The reference that weights are taken against, and the maximum that is left for the join. Rounded up: where a maximum is so large
+// that the difference is not exact (2^24 and more), the lift becomes smaller, and no weight leaves fp16.
+template <typename T, int SLACK>
+__device__ __forceinline__ float lifted(float m) {
+  if constexpr (kLift<T, SLACK> == 0.0f) return m;
+  return __fsub_ru(m, kLift<T, SLACK>);
+}
 
 // Per sequence, in shared memory; every value bounded.
 struct BatchTable {

@@ -191,7 +191,7 @@ struct Wide {
       const float ref = mx[i] == -INFINITY ? 0.0f : mx[i];  // nothing seen yet: every weight below is exp2(-inf)
       f[i] = ex2(m[i] - ref);
       m[i] = mx[i];
-      mx[i] = ref - kLift<T, 0>;
+      mx[i] = lifted<T, 0>(ref);
       l[i] *= f[i];
     }
 #pragma unroll
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_wide_kernel(Pr
           float* op = d.o + row * HD + 2 * (lane & 3);
 #pragma unroll
           for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(op + 8 * n) = make_float2(w.o[n][2 * e], w.o[n][2 * e + 1]);
-          if ((lane & 3) == 0) d.ml[row] = make_float2(w.m[e] - kLift<T, 0>, w.l[e]);
+          if ((lane & 3) == 0) d.ml[row] = make_float2(lifted<T, 0>(w.m[e]), w.l[e]);
         }
       }
     } else {
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS) prefix_wide_kernel(Pr
         }
         const long long row = d.row(r);
         d.o[row * HD + e] = o;
-        if (e == 0) d.ml[row] = make_float2(mm - kLift<T, 0>, l);
+        if (e == 0) d.ml[row] = make_float2(lifted<T, 0>(mm), l);
       }
     }
     if (i + 1 < count) {
@@ -559,8 +559,9 @@ struct Narrow {
         f[n][e] = ex2(m[n][e] - ref);
         moved |= f[n][e] != 1.0f;
         m[n][e] = mx;
-        s[n][e] = ex2(s[n][e] - (ref - kLift<T, 0>));
-        s[n][2 + e] = ex2(s[n][2 + e] - (ref - kLift<T, 0>));
+        const float against = lifted<T, 0>(ref);
+        s[n][e] = ex2(s[n][e] - against);
+        s[n][2 + e] = ex2(s[n][2 + e] - against);
         l[n][e] = fmaf(l[n][e], f[n][e], s[n][e] + s[n][2 + e]);
       }
     }
@@ -805,7 +806,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Cfg<HD>::CTAS)
         const long long row = d.row(r);
         *reinterpret_cast<float4*>(d.o + row * HD + e) = o;
         // a row whose work gave up is NaN
-        if (e == 0) d.ml[row] = make_float2(mm - kLift<T, 0>, *fail ? __int_as_float(0x7fffffff) : l);
+        if (e == 0) d.ml[row] = make_float2(lifted<T, 0>(mm), *fail ? __int_as_float(0x7fffffff) : l);
       }
       if (i + 1 < count) {
         fence_async_smem();

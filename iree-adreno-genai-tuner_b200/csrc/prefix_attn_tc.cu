@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        const float ref = (m == -INFINITY ? 0.0f : m) - kLift<T, kSlack>;
+        const float ref = lifted<T, kSlack>(m == -INFINITY ? 0.0f : m);
         const uint64_t scale = pair(a.scale2, a.scale2), off = pair(-ref, -ref);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      if (on) d.ml[at] = make_float2(m - kLift<T, kSlack>, l);
+      if (on) d.ml[at] = make_float2(lifted<T, kSlack>(m), l);
       tc_fence_before();  // O has been read: the next item's first PV waits for this half's P
       tiles += n;
       if (n > 0) x += n + 1, ++items;

@@ -463,3 +463,30 @@ def test_append_and_verify_malformed_offsets_and_guards(q4b, offsets):  # noqa: 
     n = lambda t: t.cpu().numpy()  # noqa: E731
     want, kept = R.verify(n(target), n(draft), n(tokens), n(uniforms), q_start)
     assert acc.tolist() == kept and new.t.tolist() == [77 if w is None else w for w in want]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("factor", [100.0, 230.0, 1000.0])
+@pytest.mark.parametrize("lens,prefix,H,Hkv,hd,page", [
+    ([(1, 300), (1, 9)], 0, 4, 1, 128, 16), ([(3, 300)], 0, 8, 2, 64, 16), ([(2, 300)], 0, 8, 2, 64, 20), ([(30, 300)], 0, 4, 2, 32, 16),
+    ([(1, 1)] * 40, 4000, 8, 2, 128, 16), ([(30, 300)], 0, 16, 2, 64, 16)])
+def test_scores_of_many_millions(q4b, lens, prefix, H, Hkv, hd, page, factor, dtype):  # noqa: F811
+    """Scores so large that fp32 steps by 1/2 to 4 beside them, in base 2: the key with the largest has all the weight, and the
+    result is its V, but for one rounding of the weight and one of the result."""
+    n_pages = -(-prefix // page) + sum(-(-o // page) for _, o in lens)
+    b = R.make_batch(lens, page, n_pages, prefix_len=prefix)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    kp = torch.zeros(n_pages, page, Hkv, hd, dtype=dtype, device=DEV)
+    vp = torch.randn(n_pages, page, Hkv, hd, generator=g, device=DEV).to(dtype)
+    kp[..., 0] = 30720.0
+    q = torch.zeros(b["rows"], H, hd, dtype=dtype, device=DEV)
+    q[:, :, 0] = factor
+    d = _dev(b)
+    want = torch.empty(b["rows"], H, hd, dtype=dtype, device=DEV)
+    for i, (n, o) in enumerate(lens):
+        pages, at = (b["prefix_pages"], prefix // 3) if prefix else (b["page_table"][i], (o - n) // 2)
+        kp[pages[at // page], at % page, :, 0] = 40960.0
+        want[b["q_start"][i]:b["q_start"][i + 1]] = vp[pages[at // page], at % page].repeat_interleave(H // Hkv, 0)
+    got = q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"], scale=1.0)
+    err = (got.view(want.shape).float() - want.float()).abs()
+    assert bool((err <= (torch.finfo(dtype).eps + 2.0**-15) * want.float().abs()).all())
