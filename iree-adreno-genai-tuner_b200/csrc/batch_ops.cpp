@@ -1,8 +1,9 @@
 // The batched serving operators for torch tensors, as a CPython module (q4b._batch_ops): argument checks, the
 // output and workspace allocations and the call into libq4b.so, without per-argument Python work. A step of
 // single tokens runs for a few microseconds on the GPU; the same checks in Python with ctypes took 50-65 us of host time
-// a call, this module takes a few. Refused arguments raise ValueError; a library error comes back as its
-// negative code, which the Python side turns into Q4BError with the library's message; torch's errors keep their types.
+// a call, this module takes 5 (10 to 15 for the attention, with two or three launches and its tensor maps). Refused
+// arguments raise ValueError; a library error comes back as its negative code, which the Python side turns into Q4BError
+// with the library's message; torch's errors keep their types.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 

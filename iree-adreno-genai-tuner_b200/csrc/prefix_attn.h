@@ -41,8 +41,9 @@ constexpr int kTcRows = 256, kTcKeys = 128, kTcCtas = 148;
 constexpr int kTcWholeTiles = 8;  // own items of up to so many tiles are not cut between CTAs
 constexpr int kMmKeys = 64;
 constexpr int kTcMaxBatch = 2048;  // the sequences' table shares the tensor-core kernel's shared memory
-// Prefix tiles of 16 rows x 64 keys from which the tensor-core kernel pays off. 32 rows of 3 heads behind 512 keys (384
-// tiles): 25.2 us without it, 25.4 with; behind 2048 (1536 tiles): 32.6 and 28.7.
+// Prefix tiles of 16 rows x 64 keys from which the tensor-core kernel takes them. 32 single tokens of 3 heads a KV head, 60 own
+// keys each: behind 768 keys (576 tiles) 17.3 us with it and 19.8 without, behind 2048 (1536) 20.0 and 31.3. The line was drawn
+// for the kernels one behind the other; side by side it pays from fewer tiles on (512 keys, 384 tiles: 16.5 and 18.7).
 constexpr int kTcMinUnits = 500;
 constexpr int kTcMinRows = 64;     // rows x heads of a sequence from which it takes the own keys
 

@@ -303,30 +303,45 @@ def test_append_rotates_q_in_place(q4b, layout, rows, fused):  # noqa: F811
 # ---- prefix_attention: which kernels run ------------------------------------------------------------------
 
 
-def _kernels(call):
-    from torch.profiler import ProfilerActivity, profile
-    call()
-    torch.cuda.synchronize()
-    with profile(activities=[ProfilerActivity.CUDA]) as prof:
-        call()
-        torch.cuda.synchronize()
-    return [e.key for e in prof.key_averages() if "prefix_" in e.key]
+@pytest.fixture(scope="module")
+def kernels():
+    """The kernels of some calls, by torch's profiler in a process of its own (one profiler session can leave the next one in the
+    same process without events)."""
+    import json
+    import pathlib
+    import subprocess
+    import sys
+    here = pathlib.Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, str(here / "batch_kernels_worker.py")], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return json.loads(r.stdout.strip().splitlines()[-1])
+
+
+def _steps():
+    """Steps with many rows: name -> (arguments of _attend_case, keyword arguments of the call)."""
+    many = ([(20, 70), (30, 40), (1, 8)], 16, 6000, 16, 8)
+    chunk = ([(180, 700), (1, 90)] + [(0, 5)] * 190, 16, 0, 16, 4, 64, torch.float16)
+    got = {f"many {hd} {dtype}": ((*many, hd, dtype), {}) for hd in (64, 128) for dtype in (torch.float16, torch.bfloat16)}
+    return {**got, "chunk told": (chunk, dict(max_new=180)), "chunk as single tokens": (chunk, dict(max_new=1))}
+
+
+def _odd(q):
+    """q where the tensor-core kernel does not read it: rows that do not begin at 16 bytes."""
+    rows, H, hd = q.shape
+    return torch.empty(rows, H * hd + 2, dtype=q.dtype, device=DEV)[:, 2:].view(rows, H, hd).copy_(q)
 
 
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_many_rows_run_on_the_tensor_core_kernel(q4b, hd, dtype):  # noqa: F811
+def test_many_rows_run_on_the_tensor_core_kernel(q4b, kernels, hd, dtype):  # noqa: F811
     """In this build the tensor-core kernel has the registers of its split, so the plan uses it; and a step that it is not
     used for (here for its q) runs on the other kernels with the same results."""
-    b, q, kp, vp = _attend_case([(20, 70), (30, 40), (1, 8)], 16, 6000, 16, 8, hd, dtype, 5)
-    d = _dev(b)
-    odd = torch.empty(b["rows"], 16 * hd + 2, dtype=dtype, device=DEV)[:, 2:].view(b["rows"], 16, hd)
-    odd.copy_(q)
-    call = lambda x: q4b.prefix_attention(x, kp, vp, d["prefix_pages"], 6000, d["page_table"], d["seq_lens"], d["q_start"])  # noqa: E731
-    on, off = _kernels(lambda: call(q)), _kernels(lambda: call(odd))
+    name = f"many {hd} {dtype}"
+    on, off = kernels[name], kernels[name + " odd"]
     assert any("prefix_tc_kernel" in k for k in on), on
     assert not any("prefix_tc_kernel" in k for k in off) and any("prefix_narrow_kernel" in k for k in off), off
-    _run_attend(q4b, (b, odd, kp, vp), 16)
+    b, q, kp, vp = _attend_case(*_steps()[name][0], 5)
+    _run_attend(q4b, (b, _odd(q), kp, vp), 16)
 
 
 @pytest.mark.parametrize("lens,prefix,width", [
@@ -354,12 +369,9 @@ def test_told_lengths_change_no_result(q4b, lens, prefix, width):  # noqa: F811
             q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"], **bad)
 
 
-def test_a_told_prompt_chunk_runs_on_the_tensor_cores(q4b):  # noqa: F811
-    b, q, kp, vp = _attend_case([(180, 700), (1, 90)] + [(0, 5)] * 190, 16, 0, 16, 4, 64, torch.float16, 5)
-    d = _dev(b)
-    call = lambda **kw: q4b.prefix_attention(q, kp, vp, d["prefix_pages"], 0, d["page_table"], d["seq_lens"], d["q_start"], **kw)  # noqa: E731
-    assert any("prefix_tc_kernel" in k for k in _kernels(lambda: call(max_new=180)))
-    assert not any("prefix_tc_kernel" in k for k in _kernels(lambda: call(max_new=1)))
+def test_a_told_prompt_chunk_runs_on_the_tensor_cores(kernels):
+    assert any("prefix_tc_kernel" in k for k in kernels["chunk told"])
+    assert not any("prefix_tc_kernel" in k for k in kernels["chunk as single tokens"])
 
 
 # ---- malformed offsets, with guards around everything that a call may write -------------------------------
