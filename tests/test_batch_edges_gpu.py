@@ -502,3 +502,60 @@ def test_scores_of_many_millions(q4b, lens, prefix, H, Hkv, hd, page, factor, dt
     got = q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"], scale=1.0)
     err = (got.view(want.shape).float() - want.float()).abs()
     assert bool((err <= (torch.finfo(dtype).eps + 2.0**-15) * want.float().abs()).all())
+
+
+# ---- steps one behind the other -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("B,new,prefix,H,Hkv,hd", [(32, 1, 2048, 24, 8, 128), (40, 4, 3000, 16, 4, 64), (6, 60, 500, 8, 2, 128), (20, 2, 0, 8, 2, 64)])
+def test_steps_in_a_row_see_what_the_last_one_wrote(q4b, B, new, prefix, H, Hkv, hd, graph):  # noqa: F811
+    """Decode steps without a pause: projections, lengths and offsets change in the same tensors right in front of each append, and
+    the attention of each step (two kernels that overlap, started early) gives the bits of a step that waits for everything."""
+    page, steps, rows = 16, 12, B * new
+    n_prefix, width = -(-prefix // page), -(-(40 + steps * new) // page)
+    g = torch.Generator(device=DEV).manual_seed(B)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV).half()  # noqa: E731
+    i32 = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device=DEV)  # noqa: E731
+    rng = np.random.default_rng(B)
+    ids = rng.permutation(n_prefix + B * width)
+    pages, table = i32(ids[:n_prefix]), i32(ids[n_prefix:].reshape(B, width))
+    pools = [rn(len(ids), page, Hkv, hd) for _ in range(2)]
+    qkv = [rn(rows, (H + 2 * Hkv) * hd) for _ in range(steps)]
+    news = [rng.integers(0, new + 1, B) for _ in range(steps)]  # a step's rows, some sequences idle
+    first = rng.integers(1, 40, B)
+    starts = [i32(np.concatenate([[0], np.cumsum(n)])) for n in news]
+    lens = [i32(first + np.sum(news[:s + 1], 0)) for s in range(steps)]
+    now = dict(qkv=torch.empty_like(qkv[0]), start=torch.empty_like(starts[0]), lens=torch.empty_like(lens[0]),
+               q=torch.empty(rows, H, hd, dtype=torch.float16, device=DEV))
+
+    def run(kp, vp, s, wait):
+        done = torch.cuda.synchronize if wait else lambda: None
+        now["q"].zero_()  # rows of no sequence are an input too: they share warps, and so roundings, with others
+        for name, src in (("qkv", qkv), ("start", starts), ("lens", lens)):
+            now[name].copy_(src[s])
+        done()
+        q, k, v = (x.view(rows, -1, hd) for x in now["qkv"].split([H * hd, Hkv * hd, Hkv * hd], 1))
+        q4b.paged_rope_append(q, k, v, kp, vp, table, now["lens"], now["start"], prefix_len=prefix, q_out=now["q"])
+        done()
+        return q4b.prefix_attention(now["q"], kp, vp, pages, prefix, table, now["lens"], now["start"],
+                                    out=torch.zeros(rows, H * hd, dtype=torch.float16, device=DEV))
+
+    slow = [x.clone() for x in pools]
+    want = [run(*slow, s, True).clone() for s in range(steps)]
+    fast = [x.clone() for x in pools]
+    torch.cuda.synchronize()
+    if graph:
+        cg = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(cg):
+            got = [run(*fast, s, False) for s in range(steps)]
+        for _ in range(3):
+            for x, y in zip(fast, pools):
+                x.copy_(y)
+            cg.replay()
+    else:
+        got = [run(*fast, s, False) for s in range(steps)]
+    torch.cuda.synchronize()
+    for s in range(steps):
+        assert torch.equal(got[s], want[s]), s
+    assert all(torch.equal(x, y) for x, y in zip(fast, slow))
