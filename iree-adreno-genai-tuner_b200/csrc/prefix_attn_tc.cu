@@ -505,9 +505,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         const float top = best * a.scale2;
-        if (__any_sync(0xffffffffu, top > m + kSlack || (m == -INFINITY && top > m))) {
-          const float nm = fmaxf(m, top), f = m == -INFINITY ? 0.0f : ex2(m - nm);
-          m = nm;
+        // a row's reference moves for its own maximum only: its roundings do not depend on the rows beside it
+        const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, grows)) {
+          const float f = !grows ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+          if (grows) m = top;
           l *= f;
           if (j > 0) {  // PV of the tile before has ended: its S followed it
 #pragma unroll 1

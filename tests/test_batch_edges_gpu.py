@@ -531,7 +531,6 @@ def test_steps_in_a_row_see_what_the_last_one_wrote(q4b, B, new, prefix, H, Hkv,
 
     def run(kp, vp, s, wait):
         done = torch.cuda.synchronize if wait else lambda: None
-        now["q"].zero_()  # rows of no sequence are an input too: they share warps, and so roundings, with others
         for name, src in (("qkv", qkv), ("start", starts), ("lens", lens)):
             now[name].copy_(src[s])
         done()
@@ -559,3 +558,17 @@ def test_steps_in_a_row_see_what_the_last_one_wrote(q4b, B, new, prefix, H, Hkv,
     for s in range(steps):
         assert torch.equal(got[s], want[s]), s
     assert all(torch.equal(x, y) for x, y in zip(fast, slow))
+
+
+@pytest.mark.parametrize("B,new,prefix,H,Hkv,hd", [(27, 1, 2048, 24, 8, 128), (37, 1, 3000, 24, 8, 64), (9, 40, 0, 8, 2, 128),
+                                                   (12, 3, 60, 8, 2, 64), (9, 3, 60, 8, 2, 32)])
+def test_padding_rows_change_no_bit_of_others(q4b, B, new, prefix, H, Hkv, hd):  # noqa: F811
+    """What q holds in rows of no sequence: zeros, numbers, large ones, NaN, infinities."""
+    b, q, kp, vp = _attend_case([(new, 40)] * B, 16, prefix, H, Hkv, hd, torch.float16, 1, spare=30)
+    d, n = _dev(b), B * new
+    got = []
+    for pad in (torch.zeros_like(q[n:]), 3 * torch.randn_like(q[n:]), 200 * torch.randn_like(q[n:]), float("nan"), float("inf")):
+        q[n:] = pad
+        got.append(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"])[:n].clone())
+    for x in got[1:]:
+        assert torch.equal(x, got[0])
