@@ -954,11 +954,11 @@ int prefix_units(int rows, int g, int Hkv, int prefix_len, int tr, int tk) {
   return Hkv * ((rows * g + tr - 1) / tr) * ((prefix_len + tk - 1) / tk);
 }
 
-Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv, bool wide_q) {
+Plan plan(int rows, int H, const q4b_batch& b, const q4b_paged_kv& kv, bool tensor_cores) {
   constexpr int kAll = 0x7fffffff;
   const int Hkv = kv.n_kv_heads, g = H / Hkv, R = rows * g;
   Plan p = {};
-  const bool tc = prefix_tc_takes(kv) && wide_q && prefix_tc_built(kv);
+  const bool tc = prefix_tc_takes(kv) && tensor_cores;
   const bool tc_prefix = tc && prefix_units(rows, g, Hkv, b.prefix_len, 16, kMmKeys) > kTcMinUnits;
   // several rows a sequence, as told or on average: those with many are worth the tensor cores
   const bool several = b.max_new ? b.max_new > 1 : rows > b.batch;
@@ -1126,7 +1126,7 @@ using namespace q4b;
 
 extern "C" size_t q4b_prefix_attention_workspace(int rows, int n_heads, const q4b_batch* batch, const q4b_paged_kv* kv) {
   if (check("prefix_attention", rows, n_heads, batch, kv)) return 0;
-  // whichever way q turns out to be aligned
+  // whether the tensor-core kernel turns out to be used or not: that depends on q's alignment, and on the build
   return std::max(layout(plan(rows, n_heads, *batch, *kv, true), rows, n_heads, kv->head_dim).total,
                   layout(plan(rows, n_heads, *batch, *kv, false), rows, n_heads, kv->head_dim).total);
 }
@@ -1143,7 +1143,8 @@ extern "C" int q4b_prefix_attention(const void* q, long long q_stride, long long
     return set_error(Q4B_EINVAL, "%s: q must be 4-byte aligned with even strides, out 16-byte aligned", what);
   if (!(scale > 0.0f) || !(scale < INFINITY)) return set_error(Q4B_EINVAL, "%s: scale must be positive", what);
   // the tensor-core kernel reads q in 16-byte pieces
-  const Plan p = plan(rows, n_heads, *batch, *kv, aligned(q, 16) && q_stride % 8 == 0 && q_head_stride % 8 == 0);
+  const bool wide_q = aligned(q, 16) && q_stride % 8 == 0 && q_head_stride % 8 == 0;
+  const Plan p = plan(rows, n_heads, *batch, *kv, wide_q && prefix_tc_takes(*kv) && prefix_tc_built(*kv));
   const Layout w = layout(p, rows, n_heads, kv->head_dim);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < w.total)
     return set_error(Q4B_EINVAL, "%s: needs a 256-byte aligned workspace of %zu bytes", what, w.total);

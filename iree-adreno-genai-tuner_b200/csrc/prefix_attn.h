@@ -56,7 +56,8 @@ __host__ __device__ inline int page_box(int page_size, int tile) {
 
 // whether the kernels that load by TMA can read this cache
 bool prefix_tc_takes(const q4b_paged_kv& kv);
-// whether the tensor-core kernel is as its register split needs it
+// whether the tensor-core kernel is as its register split needs it (asks the runtime); a build where it is not leaves all
+// items to the other kernels
 bool prefix_tc_built(const q4b_paged_kv& kv);
 int prefix_tc_run(const PrefixArgs& a, cudaStream_t st);
 unsigned prefix_tc_status(bool reset);

@@ -619,19 +619,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
-// The registers that the kernel was compiled to; -1 where the runtime cannot tell (no device).
+// Whether the kernel was compiled to the launch registers that its split (setmaxnreg) was laid out for. Asked once.
 template <typename T, int HD>
-int registers() {
-  static std::atomic<int> known{-1};
-  int regs = known.load(std::memory_order_relaxed);
-  if (regs < 0) {
+bool built() {
+  static std::atomic<int> regs{0};
+  if (!regs.load(std::memory_order_relaxed)) {
     cudaFuncAttributes f = {};
     if (cudaFuncGetAttributes(&f, prefix_tc_kernel<T, HD>) == cudaSuccess)
-      known.store(regs = f.numRegs, std::memory_order_relaxed);
+      regs.store(f.numRegs, std::memory_order_relaxed);
     else
       cudaGetLastError();
   }
-  return regs;
+  return regs.load(std::memory_order_relaxed) == kRegsLaunch;
 }
 
 template <typename T, int HD>
@@ -642,8 +641,6 @@ int launch(const PrefixArgs& a, cudaStream_t st) {
   if (int rc = make_tmap_pages(&tv, a.kv, a.kv.v, box)) return rc;
   auto kern = prefix_tc_kernel<T, HD>;
   static std::atomic<unsigned long long> done;
-  if (const int regs = registers<T, HD>(); regs != kRegsLaunch)  // the plan asked already, unless the runtime could not tell then
-    return set_error(Q4B_EUNSUPPORTED, "prefix_attention: built with %d registers, not %d", regs, kRegsLaunch);
   const int table = a.tc.own_lo < a.tc.own_hi ? 12 * (a.b.batch + 1) : 0;
   cudaError_t e = set_max_dynamic_smem(kern, TcCfg<HD>::SMEM + 12 * (kTcMaxBatch + 1), done);
   if (e == cudaSuccess) e = launch_pdl(kern, dim3(a.tc_ctas), dim3(kTcThreads), TcCfg<HD>::SMEM + table, st, tk, tv, a);
@@ -662,13 +659,10 @@ bool prefix_tc_takes(const q4b_paged_kv& kv) {
   return kv.head_dim >= 64 && kv.page_size % 8 == 0 && strides;
 }
 
-// The register split (setmaxnreg) needs the launch registers that it was laid out for: a compiler that gives the kernel others
-// leaves all items to the other kernels.
 bool prefix_tc_built(const q4b_paged_kv& kv) {
   const bool h16 = kv.dtype == Q4B_F16;
-  const int regs = kv.head_dim == 128 ? (h16 ? registers<__half, 128>() : registers<__nv_bfloat16, 128>())
-                                      : (h16 ? registers<__half, 64>() : registers<__nv_bfloat16, 64>());
-  return regs < 0 || regs == kRegsLaunch;
+  if (kv.head_dim == 128) return h16 ? built<__half, 128>() : built<__nv_bfloat16, 128>();
+  return h16 ? built<__half, 64>() : built<__nv_bfloat16, 64>();
 }
 
 int prefix_tc_run(const PrefixArgs& a, cudaStream_t st) {
