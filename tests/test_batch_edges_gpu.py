@@ -490,7 +490,7 @@ def test_scores_of_many_millions(q4b, lens, prefix, H, Hkv, hd, page, factor, dt
     g = torch.Generator(device=DEV).manual_seed(1)
     kp = torch.zeros(n_pages, page, Hkv, hd, dtype=dtype, device=DEV)
     vp = torch.randn(n_pages, page, Hkv, hd, generator=g, device=DEV).to(dtype)
-    kp[..., 0] = 30720.0
+    kp[..., 0] = 30464.0
     q = torch.zeros(b["rows"], H, hd, dtype=dtype, device=DEV)
     q[:, :, 0] = factor
     d = _dev(b)
