@@ -212,7 +212,7 @@ typedef struct q4b_batch {
   long long table_stride;
   int prefix_len;
   /* What the caller knows of a step without a look at the device, 0: not known. The attention's choice of kernels and SMs goes
-   * by them, its results do not. */
+   * by them, and its results only as far as sums round in another order. */
   int max_new;  /* most rows of any sequence. Not known: 1 if rows <= batch, so a prompt chunk among idle sequences wants it */
   int own_keys; /* own keys of a sequence, about. Not known: half of what a row of the table holds, so a wide table wants it */
 } q4b_batch;
@@ -255,7 +255,7 @@ int q4b_prefix_attention(const void* q, long long q_stride, long long q_head_str
                          float scale, const int32_t* prefix_pages, const q4b_batch* batch, const q4b_paged_kv* kv,
                          void* out, void* workspace, size_t workspace_bytes, q4b_stream_t stream);
 
-/* The longest that a wait in the attention kernels of calls from now on may take, in ns (1e9 unless set; captured graphs keep
+/* The longest that a wait in the attention kernels of calls from now on may take, in ns (1e9 unless set, at most 1e10; captured graphs keep
  * theirs). Rows whose work gave up are NaN, and q4b_device_status reports Q4B_ETIMEOUT. With 0 every wait gives
  * up, which shows a caller's handling of that report without a fault. */
 void q4b_prefix_attention_wait_limit(unsigned long long ns);

@@ -1176,4 +1176,6 @@ extern "C" int q4b_prefix_attention(const void* q, long long q_stride, long long
   }
 }
 
-extern "C" void q4b_prefix_attention_wait_limit(unsigned long long ns) { g_wait_ns.store(ns, std::memory_order_relaxed); }
+extern "C" void q4b_prefix_attention_wait_limit(unsigned long long ns) {
+  g_wait_ns.store(std::min(ns, 10 * (unsigned long long)kWaitLimitNs), std::memory_order_relaxed);
+}

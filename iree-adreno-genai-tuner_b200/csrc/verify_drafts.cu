@@ -5,8 +5,8 @@
 //   w = max(p - d, 0) of that row (p of the last row if all were kept): the first j with W_j > u W_{V-1}, W the
 //   running sum of w.
 //
-// The sums have 40 bits and more (64-bit words, and pairs of fp32 words over 16 values at a time): a running sum of 10^5 probabilities in fp32 is off by more than a typical w, and the
-// drawn index would depend on the order of the sum. The products u d of the tests are exact in 64 bits.
+// The sums have 40 bits and more (64-bit words, and pairs of fp32 words over 16 values at a time): a running sum of 10^5
+// probabilities in fp32 is off by more than a typical w, and the drawn index would depend on the order of the sum. The products u d of the tests are exact in 64 bits.
 //
 // Bound by memory: one row of p, and of d where a draft was rejected, per sequence; the acceptance tests read
 // two numbers per draft. A cluster of CTAs takes one sequence, so that a row's read is spread over several
@@ -78,9 +78,9 @@ __device__ __forceinline__ void unpack16(const uint4& v, float (&x)[N]) {
 // itself an fp32 number, found by Dekker's fast two-sum (of numbers a >= b >= 0, s = a + b: b - (s - a), and s = a - b:
 // (a - s) - b); the errors are added up in `lo`, which rounds too. With u = 2^-24 and S the sum of n values, an error is
 // at most u S, those of the differences together u S, so |lo| <= (k + 1) u S after k values, and the roundings of lo and of
-// its addends together u^2 S (n^2 / 2 + 5 n / 2 + 1): 169 u^2 S < 2^-40 S for n = 16. (Not emptied, over the 2048 values a lane
-// that 2^20 values on 16 warps make, equal values far below one large one put the drawn index several tokens off.) Conversions to 64 bits and
-// 64-bit additions for every value took three times as long as the row's read.
+// its addends together u^2 S (n^2 / 2 + 5 n / 2 + 1): 169 u^2 S < 2^-40 S for n = 16. (Not emptied, over the 2048 values a
+// lane that 2^20 values on 16 warps make, equal values far below one large one put the drawn index several tokens off.)
+// Conversions to 64 bits and 64-bit additions for every value took three times as long as the row's read.
 constexpr int kFlush = 16;
 struct Sum2 {
   double sum = 0.0;

@@ -65,7 +65,7 @@ def prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, page_ta
     prefix and b's own keys up to its own; a row that sees none is zero. The prefix is read
     once for all sequences. scale defaults to 1 / sqrt(hd). head_dim 32, 64 or 128.
 
-    max_new and own_keys, where the caller knows them, choose among kernels and change no result: the most rows of any
+    max_new and own_keys, where the caller knows them, choose among kernels (results differ by the order of sums alone): the most rows of any
     sequence (else 1 if rows <= B, so a step of one prompt chunk and many idle sequences wants it), and about how many
     own keys a sequence has (else half of what a row of page_table holds, so tables much wider than the sequences want it)."""
     r = (_OPS or _ops()).prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, seq_lens, q_start,
