@@ -572,3 +572,62 @@ def test_padding_rows_change_no_bit_of_others(q4b, B, new, prefix, H, Hkv, hd): 
         got.append(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"])[:n].clone())
     for x in got[1:]:
         assert torch.equal(x, got[0])
+
+
+# ---- calls of real length, and orders that are allowed ------------------------------------------------------
+
+
+def _attend64(q, kp, vp, b, page):
+    """The 64-bit form on the GPU, a sequence at a time; every page is there."""
+    rows, H, hd = q.shape
+    Hkv = kp.shape[2]
+    pick = lambda pool, pages, n: pool[torch.from_numpy(np.asarray(pages)).long().to(DEV)].reshape(-1, Hkv, hd)[:n].double()  # noqa: E731
+    out = torch.full((rows, H, hd), float("nan"), dtype=torch.float64, device=DEV)
+    p = b["prefix_len"]
+    for i, n in enumerate(b["seq_lens"].tolist()):
+        lo, hi = int(b["q_start"][i]), int(b["q_start"][i + 1])
+        own = b["page_table"][i][:-(-n // page)]
+        k, v = (torch.cat([pick(x, b["prefix_pages"], p), pick(x, own, n)]) for x in (kp, vp))
+        at = torch.arange(p + n, device=DEV)
+        for t in range(lo, hi, 64):  # some rows at a time
+            r = torch.arange(t, min(t + 64, hi), device=DEV)
+            s = torch.einsum("thgd,khd->hgtk", q[r].double().view(len(r), Hkv, H // Hkv, hd), k) / hd**0.5
+            s.masked_fill_(at > (p + n - (hi - lo) + r - lo)[:, None], -torch.inf)
+            out[r] = torch.einsum("hgtk,khd->thgd", s.softmax(-1), v).reshape(len(r), H, hd)
+    return out.cpu().numpy()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,prefix,H,Hkv,hd,page", [
+    ([(2600, 2600)], 0, 8, 2, 128, 16),  # the fill of a prefix: causal rows only
+    ([(1, 100_000), (3, 40_001)], 0, 8, 2, 64, 16),  # long own contexts
+    ([(700, 33_000), (1, 20_000)], 1000, 8, 2, 128, 64),
+    ([(5, 12_345)] * 3, 0, 8, 8, 32, 20),
+])
+def test_attend_long(q4b, lens, prefix, H, Hkv, hd, page, dtype):  # noqa: F811
+    b, q, kp, vp = _attend_case(lens, page, prefix, H, Hkv, hd, dtype, 17)
+    d = _dev(b)
+    ref = _attend64(q, kp, vp, b, page)
+    got = _f64(q4b.prefix_attention(q, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"]))
+    _check_attend(got.reshape(ref.shape), ref, _f64(vp[:64]), dtype, np.ones(len(ref), dtype=bool))
+
+
+@pytest.mark.parametrize("lens,prefix,H,Hkv,hd,page", [([(1, 30)] * 70, 4000, 8, 2, 128, 16), ([(90, 300), (2, 40)], 100, 8, 2, 64, 16),
+                                                       ([(2, 30)] * 5, 60, 8, 2, 64, 16), ([(20, 30)] * 5, 60, 8, 2, 32, 20)])
+def test_attend_orders_of_q_shared_pages_and_out_over_q(q4b, lens, prefix, H, Hkv, hd, page):  # noqa: F811
+    """In every kernel: q head-major or one row for all, pages that several places of the tables name, and the result over q."""
+    b, q, kp, vp = _attend_case(lens, page, prefix, H, Hkv, hd, torch.float16, 23)
+    kp, vp = kp.nan_to_num(0.0), vp.nan_to_num(0.0, 0.0, 0.0)
+    b["prefix_pages"][1::2] = b["prefix_pages"][::2][:len(b["prefix_pages"][1::2])]
+    b["page_table"][:] = b["page_table"][0]  # every sequence in the first one's pages
+    b["page_table"][:, -1] = b["page_table"][0, 0]
+    d = _dev(b)
+    call = lambda x, **kw: q4b.prefix_attention(x, kp, vp, d["prefix_pages"], prefix, d["page_table"], d["seq_lens"], d["q_start"], **kw)  # noqa: E731
+    ref = _attend64(q, kp, vp, b, page)
+    want = call(q)
+    _check_attend(_f64(want).reshape(ref.shape), ref, _f64(vp), torch.float16, np.ones(len(ref), dtype=bool))
+    assert torch.equal(call(q.transpose(0, 1).contiguous().transpose(0, 1)), want)
+    assert torch.equal(call(q[:1].expand_as(q)), call(q[:1].expand_as(q).contiguous()))
+    q2 = q.clone()
+    out = q2.view(len(q2), -1)
+    assert call(q2, out=out) is out and torch.equal(out, want)
